@@ -40,7 +40,7 @@ typedef void* rlpyt_stream_t; /* hipStream_t */
 const char* rlpyt_hip_last_error(void);
 /* ABI version of this header (3); bumped when a signature, an entry point or a workspace layout
  * changes, so that a stale .so fails the binding's version check instead of an attribute lookup. */
-#define RLPYT_HIP_ABI_VERSION 17
+#define RLPYT_HIP_ABI_VERSION 18
 int rlpyt_hip_abi_version(void);
 /* Fills name (<= cap bytes) with the device's gcnArchName; returns CU count or <0. */
 int rlpyt_hip_device_info(char* name, int cap);
@@ -829,6 +829,61 @@ int rlpyt_clip_adam_step_mirror_f32(const rlpyt_adam_tensor* tensors_host, int n
                                     int64_t* tick_ctr /*nullable*/, int mirror_index,
                                     float* mirror_pt /*nullable*/, int64_t mirror_rows,
                                     int64_t mirror_cols, rlpyt_stream_t stream);
+
+/* ---- training a recurrent policy over long sequences (no counterpart in the reference) ------------------
+ * dtype: 0 = f32, 1 = bf16, 2 = f16 (of the streams, logits and matrices; everything declared float* is f32). */
+
+/* Gated linear recurrence over [T, B, D], unit stride along D, element strides *_ts along T and *_bs along B:
+ *   z = sigmoid(gate)    h_t = (1 - z_t) k_t h_{t-1} + z_t x_t    k = 0 where reset [T,B] (u8, may be null), else 1
+ * h0 [B,D] (null: 0), lengths [B] (null: T; clamped to 0 .. T): a sequence's steps from lengths[b] on are not
+ * used, their h is 0 and its state stays.  hn [B,D] (may be null): the state after the last step.  states (may be
+ * null; [rlpyt_gated_scan_state_rows(T), B, D]): what the backward pass needs.  workspace:
+ * rlpyt_gated_scan_workspace_bytes, for either direction.
+ * Backward: dh strides may be 0; dhn may be null; dx, dgate 0 behind a sequence's end; dh0 may be null. */
+int64_t rlpyt_gated_scan_state_rows(int64_t T);
+int64_t rlpyt_gated_scan_workspace_bytes(int64_t T, int64_t B, int64_t D);
+int rlpyt_gated_scan_fwd(int dtype, const void* x, int64_t x_ts, int64_t x_bs, const void* gate, int64_t g_ts,
+                         int64_t g_bs, const float* h0, const uint8_t* reset, const int64_t* lengths, void* h,
+                         int64_t h_ts, int64_t h_bs, float* hn, float* states, int64_t T, int64_t B, int64_t D,
+                         void* workspace, rlpyt_stream_t stream);
+int rlpyt_gated_scan_bwd(int dtype, const void* x, int64_t x_ts, int64_t x_bs, const void* gate, int64_t g_ts,
+                         int64_t g_bs, const void* dh, int64_t d_ts, int64_t d_bs, const float* dhn,
+                         const uint8_t* reset, const int64_t* lengths, const float* states, void* dx,
+                         int64_t dx_ts, int64_t dx_bs, void* dgate, int64_t dg_ts, int64_t dg_bs, float* dh0,
+                         int64_t T, int64_t B, int64_t D, void* workspace, rlpyt_stream_t stream);
+/* One step: state [B,D] dense, f32, updated in place; y [B,D] dense; reset [B] u8 or null. */
+int rlpyt_gated_scan_step(int dtype, const void* x, int64_t x_bs, const void* gate, int64_t g_bs,
+                          const uint8_t* reset, float* state, void* y, int64_t B, int64_t D,
+                          rlpyt_stream_t stream);
+
+/* Clipped policy loss with a KL term over softmax(logits [N,V]), rows row_stride elements apart:
+ *   r = exp(logp - old_logp)    pi = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)    d = ref_logp - logp
+ *   loss = sum valid (pi + kl_coeff (e^d - d - 1) - entropy_coeff H) / sum valid
+ * ref_logp, valid (f32 weights; rows of weight 0 are not read) may be null.  scalars [5] = loss, pi, kl, entropy
+ * and clipped share (weighted means; 0 when nothing is valid).  logp, entropy [N] (both or neither): of the
+ * rows of weight != 0.  grad [N,V] dense (may be null): d loss / d logits.  A row of -inf only adds nothing; an action
+ * outside 0 .. V-1 makes the loss NaN. */
+int64_t rlpyt_policy_loss_workspace_bytes(int dtype, int64_t N, int64_t V);
+int rlpyt_policy_kl_loss_fwd_bwd(int dtype, const void* logits, int64_t row_stride, const int64_t* action,
+                                 const float* old_logp, const float* advantage, const float* ref_logp,
+                                 const float* valid, int64_t N, int64_t V, double clip_low, double clip_high,
+                                 double kl_coeff, double entropy_coeff, float* scalars, float* logp,
+                                 float* entropy, void* grad, void* workspace, rlpyt_stream_t stream);
+/* log softmax(logits)[action] and the entropy of every row. */
+int rlpyt_action_logp(int dtype, const void* logits, int64_t row_stride, const int64_t* action, int64_t N,
+                      int64_t V, float* logp, float* entropy, void* workspace, rlpyt_stream_t stream);
+/* x *= *scale in place (x 16-byte aligned); nothing is touched where the device scalar is 1. */
+int rlpyt_scale_unless_one(int dtype, void* x, int64_t n, const float* scale, rlpyt_stream_t stream);
+
+/* Newton-Schulz orthogonalisation of n matrices (host tables; matrix i is rows[i] x cols[i], row stride ld[i],
+ * its result dense):  X = G / (|G|_F + eps),  steps x:  X <- a X + (b A + c A A) X  with  A = X X^T (of the wide
+ * form).  Products to 22 bits with f32 accumulation.  Sides up to 65536; the coefficients have to keep singular
+ * values of 0 .. 1 below sqrt(8) and the factor a + b s^2 + c s^4 below 8.  workspace:
+ * rlpyt_orthogonalize_workspace_bytes, 16-byte aligned. */
+int64_t rlpyt_orthogonalize_workspace_bytes(const int64_t* rows_host, const int64_t* cols_host, int n);
+int rlpyt_orthogonalize(int dtype, const void* const* in_host, const int64_t* ld_host, void* const* out_host,
+                        const int64_t* rows_host, const int64_t* cols_host, int n, int steps, float a, float b,
+                        float c, double eps, void* workspace, rlpyt_stream_t stream);
 
 #ifdef __cplusplus
 }

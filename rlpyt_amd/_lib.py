@@ -18,7 +18,7 @@ import torch  # noqa: F401  (must precede the CDLL load; see module docstring)
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # (RLPYT_HIP_LIB: another build of the same ABI, for A/B runs of two kernel versions on one box)
 LIB_PATH = os.environ.get("RLPYT_HIP_LIB") or os.path.join(_HERE, "csrc", "librlpyt_hip.so")
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 
 class CopyDesc(ctypes.Structure):
@@ -208,6 +208,22 @@ _SIGNATURES = {
     "rlpyt_sumtree_sample": (c_int, [_p, _p, c_int, _p, _p, _p, _p]),
     "rlpyt_sumtree_set_sampled": (c_int, [_p, _p, c_int, _p, _p]),
     "rlpyt_sumtree_update": (c_int, [_p, _p, c_int, _p]),
+    "rlpyt_gated_scan_state_rows": (c_int64, [c_int64]),
+    "rlpyt_gated_scan_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64]),
+    "rlpyt_gated_scan_fwd": (c_int, [c_int, _p, c_int64, c_int64, _p, c_int64, c_int64, _p, _p, _p, _p, c_int64,
+                                     c_int64, _p, _p, c_int64, c_int64, c_int64, _p, _p]),
+    "rlpyt_gated_scan_bwd": (c_int, [c_int, _p, c_int64, c_int64, _p, c_int64, c_int64, _p, c_int64, c_int64, _p,
+                                     _p, _p, _p, _p, c_int64, c_int64, _p, c_int64, c_int64, _p, c_int64, c_int64,
+                                     c_int64, _p, _p]),
+    "rlpyt_gated_scan_step": (c_int, [c_int, _p, c_int64, _p, c_int64, _p, _p, _p, c_int64, c_int64, _p]),
+    "rlpyt_policy_loss_workspace_bytes": (c_int64, [c_int, c_int64, c_int64]),
+    "rlpyt_policy_kl_loss_fwd_bwd": (c_int, [c_int, _p, c_int64, _p, _p, _p, _p, _p, c_int64, c_int64, c_double,
+                                             c_double, c_double, c_double, _p, _p, _p, _p, _p, _p]),
+    "rlpyt_action_logp": (c_int, [c_int, _p, c_int64, _p, c_int64, c_int64, _p, _p, _p, _p]),
+    "rlpyt_scale_unless_one": (c_int, [c_int, _p, c_int64, _p, _p]),
+    "rlpyt_orthogonalize_workspace_bytes": (c_int64, [_p, _p, c_int]),
+    "rlpyt_orthogonalize": (c_int, [c_int, _p, _p, _p, _p, _p, c_int, c_int, c_float, c_float, c_float, c_double,
+                                    _p, _p]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

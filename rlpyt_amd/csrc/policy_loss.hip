@@ -1,0 +1,580 @@
+// Clipped policy loss with a KL term and an entropy bonus over a softmax policy given by its logits [N, V],
+// forward and backward in one pass, and the log-probabilities that it takes as inputs.
+//
+//   logp = l_a - lse(l)     r = exp(logp - old_logp)     d = ref_logp - logp
+//   pi = -min(r A, clip(r, 1 - lo, 1 + hi) A)     kl = e^d - d - 1     H = -sum_j p_j log p_j
+//   loss = sum_n w_n (pi + c_kl kl - c_H H) / sum_n w_n
+//   dl_j = w / sum w [ c 1_{j = a} + p_j (c_H (log p_j + H) - c) ]     c = dpi/dlogp - c_kl (e^d - 1)
+//
+// Memory bound: the floor reads and writes the logits once.  A row is kept in registers (a group of lanes for
+// V <= 1024, a workgroup up to 256 KB a row) between the softmax statistics and the gradient.  Longer rows,
+// and batches of so few rows that one workgroup each leaves the chip idle, are split over workgroups: one
+// launch for the statistics of the parts, one that joins them and reads the row again for the gradient.
+//
+// Sums over a row are f32 per lane and in a fixed order (no atomics); log(sum) and everything per row is 64 bits:
+// kl ~ d^2 / 2 cancels in 32.  x - max is formed before it is scaled for exp2, so that the error of e^(x - max) goes with
+// its exponent and not with the logit.  A difference below -200 counts as -200 (its e^ is 0 in f32), which keeps
+// 0 * log 0 = 0 for logits of -inf; NaN goes through to the loss.
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.h"
+
+namespace rlpyt {
+namespace {
+
+template <typename E>
+struct Row16 {   // 16 bytes of a row; rows of odd length start anywhere, global loads need only the element's alignment
+  static constexpr int n = 16 / sizeof(E);
+  typedef E vec __attribute__((ext_vector_type(n)));
+  struct __attribute__((packed, aligned(sizeof(E)))) raw { vec v; };
+};
+
+struct LossArgs {
+  const void* logits;
+  int64_t row_stride;             // elements
+  const int64_t* action;
+  const float *old_logp, *advantage, *ref_logp, *valid;   // ref_logp, valid: may be null
+  void* grad;                     // [N, V] dense, or null
+  float *logp, *entropy;          // [N] each, or null
+  double* rows;                   // [n, 4]: w pi, w kl, w H, w clipped of a row (or workgroup), or null (log-probabilities only)
+  const double* denom;            // sum of valid, or null: N
+  float3* parts;                  // split rows: (max, sum, weighted sum) of the parts [N, P]
+  int64_t N, n0, n_rows;          // a launch takes the rows n0 .. n0 + n_rows - 1
+  int V, part;                    // part: elements of a row's part, a multiple of 8
+  double lo, hi, c_kl, c_ent;
+};
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kFloor = -200.f;   // e^-200 is 0 in f32
+
+__device__ __forceinline__ float below(float x, float m) {
+  const float t = x - m;
+  return t < kFloor ? kFloor : t;  // (NaN stays NaN)
+}
+__device__ __forceinline__ float exp_of(float t) { return __builtin_amdgcn_exp2f(t * kLog2e); }
+
+// Softmax statistics of some logits: s = sum e^(x - m), u = sum e^(x - m) (x - m); m = -inf: none.
+struct Stats {
+  float m, s, u;
+};
+__device__ __forceinline__ Stats join(const Stats& p, const Stats& q) {
+  Stats r;
+  r.m = fmaxf(p.m, q.m);
+  if (r.m == -INFINITY) return Stats{-INFINITY, p.s + q.s, 0.f};   // (NaN sums stay)
+  const float dp = below(p.m, r.m), dq = below(q.m, r.m), fp = exp_of(dp), fq = exp_of(dq);
+  r.s = fmaf(fp, p.s, fq * q.s);
+  r.u = fp * fmaf(dp, p.s, p.u) + fq * fmaf(dq, q.s, q.u);
+  return r;
+}
+template <int G>
+__device__ __forceinline__ Stats group_join(Stats v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) {
+    Stats q;
+    q.m = __shfl_xor(v.m, o, kWave), q.s = __shfl_xor(v.s, o, kWave), q.u = __shfl_xor(v.u, o, kWave);
+    v = join(v, q);
+  }
+  return v;
+}
+template <int G>
+__device__ __forceinline__ float group_max(float m) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
+  return m;
+}
+
+// What follows from a row's statistics: its terms of the loss, and its gradient as e^t (k1 t + k0), + ka at the action.
+struct RowOut {
+  double pi, kl, ent, clipped;
+  float logp, entropy, m, k1, k0, ka;
+};
+__device__ __forceinline__ RowOut row_terms(const LossArgs& p, int64_t n, float w, const Stats& st,
+                                            bool some, float xa, bool in_range) {
+  RowOut o = {};
+  o.m = st.m;
+  if (!some) {   // every logit is -inf: no distribution, the row adds nothing and has no gradient
+    o.m = 0.f;
+    o.logp = -INFINITY;
+    return o;
+  }
+  const double logs = log((double)st.s);
+  const double H = logs - (double)st.u / (double)st.s;
+  const double lp = in_range ? ((double)xa - (double)st.m) - logs : (double)NAN;
+  o.logp = (float)lp;
+  o.entropy = (float)H;
+  if (!p.rows) return o;
+  const double A = (double)p.advantage[n], r = exp(lp - (double)p.old_logp[n]);
+  const double rc = fmin(fmax(r, 1.0 - p.lo), 1.0 + p.hi);
+  double c = 0.0;
+  if (A != 0.0 || r != r) {
+    const double plain = r * A, clip = rc * A;
+    o.pi = -(plain < clip ? plain : clip);
+    if (plain != plain) o.pi = plain;
+    if (!(plain > clip)) c = -plain;
+  }
+  o.clipped = r != rc ? 1.0 : 0.0;
+  if (p.ref_logp) {
+    const double d = (double)p.ref_logp[n] - lp, e = expm1(d);
+    o.kl = e - d;
+    c -= p.c_kl * e;
+  }
+  o.ent = H;
+  const double denom = p.denom ? *p.denom : (double)p.N;
+  const double g = denom > 0.0 ? (double)w / denom : 0.0, gs = g / (double)st.s;
+  o.k1 = (float)(gs * p.c_ent);
+  o.k0 = (float)(gs * (p.c_ent * (H - logs) - c));
+  o.ka = (float)(g * c);
+  o.pi *= w, o.kl *= w, o.ent *= w, o.clipped *= w;
+  return o;
+}
+
+// ---- V <= 16 G: G lanes a row, K elements a lane ---------------------------------------------------------
+template <typename E, int G, int K>
+__global__ __launch_bounds__(256) void loss_group_kernel(const LossArgs p) {
+  __shared__ double sums[4 * 16];
+  const int sub = threadIdx.x & (G - 1);
+  const int64_t n = p.n0 + (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+  const bool on = n < p.n0 + p.n_rows;
+  const float w = on ? (p.valid ? p.valid[n] : 1.f) : 0.f;
+  RowOut o = {};
+  if (on) {
+    const bool live = w != 0.f;           // padded rows are not read
+    const E* row = (const E*)p.logits + n * p.row_stride;
+    float x[K], m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int j = sub + k * G;
+      x[k] = live && j < p.V ? (float)row[j] : -INFINITY;
+      m = fmaxf(m, x[k]);
+    }
+    m = group_max<G>(m);
+    Stats st = {m, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float t = below(x[k], m == -INFINITY ? 0.f : m), e = exp_of(t);
+      st.s += e;
+      st.u = fmaf(e, t, st.u);
+    }
+#pragma unroll
+    for (int o2 = G / 2; o2 > 0; o2 >>= 1) {
+      st.s += __shfl_xor(st.s, o2, kWave);
+      st.u += __shfl_xor(st.u, o2, kWave);
+    }
+    if (live) {
+      const int64_t a = p.action[n];
+      const bool in_range = a >= 0 && a < p.V;
+      o = row_terms(p, n, w, st, !(m == -INFINITY && st.s == 0.f), in_range ? (float)row[a] : 0.f, in_range);
+      if (p.logp && sub == 0) p.logp[n] = o.logp, p.entropy[n] = o.entropy;
+    }
+    if (p.grad) {
+      E* g = (E*)p.grad + n * p.V;
+      const int64_t a = live ? p.action[n] : -1;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int j = sub + k * G;
+        const float t = below(x[k], o.m), e = exp_of(t);
+        float v = e * fmaf(o.k1, t, o.k0);
+        if (j == a) v += o.ka;
+        if (j < p.V) g[j] = (E)(live ? v : 0.f);
+      }
+    }
+  }
+  if (!p.rows) return;
+  double v[4] = {0.0, 0.0, 0.0, 0.0};
+  if (sub == 0) v[0] = o.pi, v[1] = o.kl, v[2] = o.ent, v[3] = o.clipped;
+  block_sum<4>(v, sums);
+  if (threadIdx.x == 0)
+    for (int k = 0; k < 4; ++k) p.rows[(p.n0 / (256 / G) + blockIdx.x) * 4 + k] = v[k];
+}
+
+// ---- a row held by one workgroup of NT threads, R x 16 bytes a thread -------------------------------------
+template <typename E>
+__device__ __forceinline__ typename Row16<E>::vec load16(const E* __restrict__ row, int j, int V) {
+  typedef typename Row16<E>::vec vec;
+  constexpr int n = Row16<E>::n;
+  if (j + n <= V) return reinterpret_cast<const typename Row16<E>::raw*>(row + j)->v;
+  vec v;
+#pragma unroll
+  for (int k = 0; k < n; ++k) v[k] = j + k < V ? row[j + k] : (E)-INFINITY;
+  return v;
+}
+template <typename E>
+__device__ __forceinline__ void store16(E* __restrict__ row, int j, int V, typename Row16<E>::vec v) {
+  constexpr int n = Row16<E>::n;
+  if (j + n <= V) {
+    reinterpret_cast<typename Row16<E>::raw*>(row + j)->v = v;
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < n; ++k)
+    if (j + k < V) row[j + k] = v[k];
+}
+template <typename E>
+__device__ __forceinline__ typename Row16<E>::vec grad16(typename Row16<E>::vec x, int j, int64_t a,
+                                                         const RowOut& o) {
+  constexpr int n = Row16<E>::n;
+  typename Row16<E>::vec v;
+#pragma unroll
+  for (int k = 0; k < n; ++k) {
+    const float t = below((float)x[k], o.m), e = exp_of(t);
+    float g = e * fmaf(o.k1, t, o.k0);
+    if (j + k == a) g += o.ka;
+    v[k] = (E)g;
+  }
+  return v;
+}
+// statistics of the vectors of a wave
+template <typename E, int R>
+__device__ __forceinline__ Stats wave_stats(const typename Row16<E>::vec (&x)[R]) {
+  constexpr int n = Row16<E>::n;
+  float m = -INFINITY;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int k = 0; k < n; ++k) m = fmaxf(m, (float)x[r][k]);
+  m = group_max<kWave>(m);
+  Stats st = {m, 0.f, 0.f};
+  const float from = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+      const float t = below((float)x[r][k], from), e = exp_of(t);
+      st.s += e;
+      st.u = fmaf(e, t, st.u);
+    }
+  st.s = wave_sum(st.s);
+  st.u = wave_sum(st.u);
+  return st;
+}
+// joins the waves' statistics; every thread gets the result
+template <int NT>
+__device__ __forceinline__ Stats block_join(const Stats& st, Stats* lds) {
+  constexpr int NW = NT / kWave;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  if (lane == 0) lds[w] = st;
+  __syncthreads();
+  Stats v = lane < NW ? lds[lane] : Stats{-INFINITY, 0.f, 0.f};
+  v = group_join<NW>(v);
+  v.m = __shfl(v.m, 0, kWave), v.s = __shfl(v.s, 0, kWave), v.u = __shfl(v.u, 0, kWave);
+  return v;
+}
+
+template <typename E, int NT, int R>
+__global__ __launch_bounds__(NT) void loss_row_kernel(const LossArgs p) {
+  typedef typename Row16<E>::vec vec;
+  constexpr int n16 = Row16<E>::n;
+  __shared__ Stats lds[NT / kWave];
+  __shared__ RowOut out;
+  const int64_t n = p.n0 + blockIdx.x;
+  const float w = p.valid ? p.valid[n] : 1.f;
+  E* g = p.grad ? (E*)p.grad + n * p.V : nullptr;
+  if (w == 0.f) {   // a padded row: not read, no gradient
+    if (g) {
+      vec zero;
+#pragma unroll
+      for (int k = 0; k < n16; ++k) zero[k] = (E)0.f;
+      for (int r = 0; r < R; ++r) {
+        const int j = (r * NT + threadIdx.x) * n16;
+        if (j < p.V) store16<E>(g, j, p.V, zero);
+      }
+    }
+    if (p.rows && threadIdx.x < 4) p.rows[n * 4 + threadIdx.x] = 0.0;
+    return;
+  }
+  const E* row = (const E*)p.logits + n * p.row_stride;
+  const int64_t a = p.action[n];
+  const bool in_range = a >= 0 && a < p.V;
+  const float xa = in_range ? (float)row[a] : 0.f;
+  vec x[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) x[r] = load16<E>(row, (r * NT + threadIdx.x) * n16, p.V);
+  const Stats st = block_join<NT>(wave_stats<E, R>(x), lds);
+  if (threadIdx.x == 0) {
+    out = row_terms(p, n, w, st, !(st.m == -INFINITY && st.s == 0.f), xa, in_range);
+    if (p.logp) p.logp[n] = out.logp, p.entropy[n] = out.entropy;
+    if (p.rows) p.rows[n * 4] = out.pi, p.rows[n * 4 + 1] = out.kl, p.rows[n * 4 + 2] = out.ent, p.rows[n * 4 + 3] = out.clipped;
+  }
+  if (!g) return;
+  __syncthreads();
+  const RowOut o = out;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int j = (r * NT + threadIdx.x) * n16;
+    if (j < p.V) store16<E>(g, j, p.V, grad16<E>(x[r], j, a, o));
+  }
+}
+
+// ---- rows split over workgroups ----------------------------------------------------------------------------
+constexpr int kSplitThreads = 256, kSplitVecs = 4;   // vectors in flight per thread
+
+template <typename E>
+__global__ __launch_bounds__(kSplitThreads) void loss_parts_kernel(const LossArgs p, int P) {
+  typedef typename Row16<E>::vec vec;
+  constexpr int n16 = Row16<E>::n, step = kSplitThreads * kSplitVecs * n16;
+  __shared__ Stats lds[kSplitThreads / kWave];
+  const int64_t n = p.n0 + blockIdx.x / P;
+  const int i = blockIdx.x % P;
+  if (p.valid && p.valid[n] == 0.f) return;
+  const E* row = (const E*)p.logits + n * p.row_stride;
+  const int begin = i * p.part, end = min(p.V, begin + p.part);
+  Stats st = {-INFINITY, 0.f, 0.f};
+  for (int j0 = begin; j0 < end; j0 += step) {
+    vec x[kSplitVecs];
+#pragma unroll
+    for (int r = 0; r < kSplitVecs; ++r) x[r] = load16<E>(row, j0 + (r * kSplitThreads + threadIdx.x) * n16, end);
+    st = join(st, wave_stats<E, kSplitVecs>(x));
+  }
+  st = block_join<kSplitThreads>(st, lds);
+  if (threadIdx.x == 0) p.parts[n * P + i] = float3{st.m, st.s, st.u};
+}
+
+template <typename E>
+__global__ __launch_bounds__(kSplitThreads) void loss_join_kernel(const LossArgs p, int P, int blocks) {
+  typedef typename Row16<E>::vec vec;
+  constexpr int n16 = Row16<E>::n, step = kSplitThreads * n16;
+  __shared__ Stats lds[kSplitThreads / kWave];
+  __shared__ RowOut out;
+  const int64_t n = p.n0 + blockIdx.x / blocks;   // blocks per row: P, or 1 without a gradient
+  const int part = blockIdx.x % blocks;
+  const float w = p.valid ? p.valid[n] : 1.f;
+  const bool live = w != 0.f;
+  const bool first = part == 0;
+  const int64_t a = live ? p.action[n] : -1;
+  const E* row = (const E*)p.logits + n * p.row_stride;
+  if (live) {
+    Stats st = {-INFINITY, 0.f, 0.f};
+    for (int i = threadIdx.x; i < P; i += kSplitThreads) {
+      const float3 q = p.parts[n * P + i];
+      st = join(st, Stats{q.x, q.y, q.z});
+    }
+    st = block_join<kSplitThreads>(group_join<kWave>(st), lds);
+    if (threadIdx.x == 0) {
+      const bool in_range = a >= 0 && a < p.V;
+      out = row_terms(p, n, w, st, !(st.m == -INFINITY && st.s == 0.f), in_range ? (float)row[a] : 0.f, in_range);
+      if (first && p.logp) p.logp[n] = out.logp, p.entropy[n] = out.entropy;
+    }
+  } else if (threadIdx.x == 0) {
+    out = RowOut{};
+  }
+  if (threadIdx.x == 0 && first && p.rows)
+    p.rows[n * 4] = out.pi, p.rows[n * 4 + 1] = out.kl, p.rows[n * 4 + 2] = out.ent, p.rows[n * 4 + 3] = out.clipped;
+  if (!p.grad) return;
+  __syncthreads();
+  const RowOut o = out;
+  E* g = (E*)p.grad + n * p.V;
+  const int begin = part * p.part, end = min(p.V, begin + p.part);
+  for (int j = begin + threadIdx.x * n16; j < end; j += step) {
+    vec v;
+    if (live) {
+      v = grad16<E>(load16<E>(row, j, end), j, a, o);
+    } else {
+#pragma unroll
+      for (int k = 0; k < n16; ++k) v[k] = (E)0.f;
+    }
+    store16<E>(g, j, end, v);
+  }
+}
+
+// ---- sums over the rows -------------------------------------------------------------------------------------
+__global__ __launch_bounds__(1024) void loss_denom_kernel(const float* __restrict__ valid, int64_t N,
+                                                          double* __restrict__ denom) {
+  __shared__ double scratch[16];
+  double v[1] = {0.0};
+  for (int64_t i = threadIdx.x; i < N; i += 1024) v[0] += (double)valid[i];
+  block_sum<1>(v, scratch);
+  if (threadIdx.x == 0) *denom = v[0];
+}
+
+__global__ __launch_bounds__(1024) void loss_finish_kernel(const double* __restrict__ rows, int64_t n,
+                                                           const double* __restrict__ denom, double N, double c_kl,
+                                                           double c_ent, float* __restrict__ scalars) {
+  __shared__ double scratch[4 * 16];
+  double v[4] = {0.0, 0.0, 0.0, 0.0};
+  for (int64_t i = threadIdx.x; i < n; i += 1024)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] += rows[i * 4 + k];
+  block_sum<4>(v, scratch);
+  if (threadIdx.x != 0) return;
+  const double d = denom ? *denom : N;
+  const double inv = d > 0.0 ? 1.0 / d : 0.0;   // nothing valid: a loss of 0
+  for (int k = 0; k < 4; ++k) v[k] *= inv;
+  scalars[0] = (float)(v[0] + c_kl * v[1] - c_ent * v[2]);
+  for (int k = 0; k < 4; ++k) scalars[1 + k] = (float)v[k];
+}
+
+// grad *= *scale, in place; nothing is read or written where *scale is 1.
+template <typename E>
+__global__ __launch_bounds__(256) void loss_scale_kernel(E* __restrict__ g, int64_t n,
+                                                         const float* __restrict__ scale) {
+  typedef typename Row16<E>::vec vec;
+  constexpr int n16 = Row16<E>::n;
+  const float f = *scale;
+  if (f == 1.f) return;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * n16;
+  if (i >= n) return;
+  if (i + n16 <= n) {
+    vec v = *reinterpret_cast<const vec*>(g + i);
+#pragma unroll
+    for (int k = 0; k < n16; ++k) v[k] = (E)((float)v[k] * f);
+    *reinterpret_cast<vec*>(g + i) = v;
+  } else {
+    for (int64_t k = i; k < n; ++k) g[k] = (E)((float)g[k] * f);
+  }
+}
+
+// ------------------------------------------------------------------------------------ host side
+enum { F32 = 0, BF16 = 1, F16 = 2 };
+constexpr int kGroupV = 1024;       // longest row of the lane groups
+
+struct LossPlan {
+  int P, part;                      // P > 0: rows split into P parts of `part` elements
+  int64_t partials;                 // rows of the [., 4] table of partial sums
+};
+int group_lanes(int64_t V) { return V <= 32 ? 8 : V <= 64 ? 16 : V <= 128 ? 32 : 64; }
+
+// A row goes to one workgroup while it fits its registers (256 KB) and the rows fill the chip; otherwise it is split into parts of
+// at least 8 KB so that there are about 1024 workgroups.  The split reads the row twice: it pays below ~128 rows.
+LossPlan plan_of(int64_t N, int64_t V, int size) {
+  LossPlan q = {0, 0, N};
+  if (V <= kGroupV) {
+    q.partials = ceil_div(N, 256 / group_lanes(V));
+    return q;
+  }
+  const bool held = V * size <= 256 * 1024;
+  if (held && (N >= 128 || V * size <= 16 * 1024)) return q;
+  const int64_t least = ceil_div(V * size, 8 * 1024), want = std::max<int64_t>(1, ceil_div(1024, N));
+  const int64_t P = std::max<int64_t>(1, std::min(least, std::max<int64_t>(want, held ? 1 : 4)));
+  q.part = (int)(ceil_div(ceil_div(V, P), 8) * 8);
+  q.P = (int)ceil_div(V, q.part);
+  return q;
+}
+
+template <typename E>
+int run(LossArgs p, const LossPlan& q, hipStream_t s) {
+  const int V = p.V;
+  if (V <= kGroupV) {
+    const dim3 grid((unsigned)ceil_div(p.n_rows, 256 / group_lanes(V)));
+    if (V <= 8) RL_LAUNCH((loss_group_kernel<E, 8, 1>), grid, dim3(256), 0, s, p);
+    else if (V <= 32) RL_LAUNCH((loss_group_kernel<E, 8, 4>), grid, dim3(256), 0, s, p);
+    else if (V <= 64) RL_LAUNCH((loss_group_kernel<E, 16, 4>), grid, dim3(256), 0, s, p);
+    else if (V <= 128) RL_LAUNCH((loss_group_kernel<E, 32, 4>), grid, dim3(256), 0, s, p);
+    else if (V <= 256) RL_LAUNCH((loss_group_kernel<E, 64, 4>), grid, dim3(256), 0, s, p);
+    else RL_LAUNCH((loss_group_kernel<E, 64, 16>), grid, dim3(256), 0, s, p);
+  } else if (q.P == 0) {
+    const dim3 grid((unsigned)p.n_rows);
+    const int64_t vecs = ceil_div((int64_t)V, (int64_t)Row16<E>::n);
+    if (vecs <= 512) RL_LAUNCH((loss_row_kernel<E, 256, 2>), grid, dim3(256), 0, s, p);
+    else if (vecs <= 1024) RL_LAUNCH((loss_row_kernel<E, 256, 4>), grid, dim3(256), 0, s, p);
+    else if (vecs <= 2048) RL_LAUNCH((loss_row_kernel<E, 512, 4>), grid, dim3(512), 0, s, p);
+    else if (vecs <= 4096) RL_LAUNCH((loss_row_kernel<E, 1024, 4>), grid, dim3(1024), 0, s, p);
+    else if (vecs <= 8192) RL_LAUNCH((loss_row_kernel<E, 1024, 8>), grid, dim3(1024), 0, s, p);
+    else RL_LAUNCH((loss_row_kernel<E, 1024, 16>), grid, dim3(1024), 0, s, p);
+  } else {
+    const int blocks = p.grad ? q.P : 1;
+    RL_LAUNCH((loss_parts_kernel<E>), dim3((unsigned)(p.n_rows * q.P)), dim3(kSplitThreads), 0, s, p, q.P);
+    RL_LAUNCH((loss_join_kernel<E>), dim3((unsigned)(p.n_rows * blocks)), dim3(kSplitThreads), 0, s, p, q.P, blocks);
+  }
+  RL_LAUNCH_CHECK();
+  return RLPYT_OK;
+}
+
+int element_size(int dtype) { return dtype == F32 ? 4 : 2; }
+
+// A launch holds less than 2^32 threads: large batches go in slices of rows.
+int64_t slice_rows(const LossPlan& q) { return q.P > 0 ? std::max<int64_t>(1, ((int64_t)1 << 22) / q.P) : (int64_t)1 << 21; }
+
+int run_all(int dtype, LossArgs p, const LossPlan& q, hipStream_t s) {
+  const int64_t slice = slice_rows(q);
+  for (p.n0 = 0; p.n0 < p.N; p.n0 += slice) {
+    p.n_rows = std::min(slice, p.N - p.n0);
+    int rc;
+    if (dtype == F32) rc = run<float>(p, q, s);
+    else if (dtype == BF16) rc = run<__bf16>(p, q, s);
+    else rc = run<_Float16>(p, q, s);
+    if (rc != RLPYT_OK) return rc;
+  }
+  return RLPYT_OK;
+}
+
+// workspace: sum of valid | 4 partial sums per row or workgroup | statistics of the parts
+int64_t parts_offset(const LossPlan& q) { return 16 + q.partials * 4 * (int64_t)sizeof(double); }
+
+}  // namespace
+}  // namespace rlpyt
+
+using namespace rlpyt;
+
+extern "C" int64_t rlpyt_policy_loss_workspace_bytes(int dtype, int64_t N, int64_t V) {
+  if (dtype < F32 || dtype > F16 || N <= 0 || V <= 0) return 16;
+  const LossPlan q = plan_of(N, V, element_size(dtype));
+  return parts_offset(q) + N * q.P * (int64_t)sizeof(float3);
+}
+
+extern "C" int rlpyt_policy_kl_loss_fwd_bwd(int dtype, const void* logits, int64_t row_stride,
+                                            const int64_t* action, const float* old_logp,
+                                            const float* advantage, const float* ref_logp, const float* valid,
+                                            int64_t N, int64_t V, double clip_low, double clip_high,
+                                            double kl_coeff, double entropy_coeff, float* scalars, float* logp,
+                                            float* entropy, void* grad, void* workspace, rlpyt_stream_t stream) {
+  RL_CHECK_ARG(dtype >= F32 && dtype <= F16, RLPYT_EINVAL, "rlpyt_policy_kl_loss_fwd_bwd: unknown dtype %d", dtype);
+  RL_CHECK_ARG(N >= 0 && V > 0 && V <= (1 << 30), RLPYT_ESHAPE,
+               "rlpyt_policy_kl_loss_fwd_bwd: N=%ld V=%ld out of range", (long)N, (long)V);
+  RL_CHECK_ARG(scalars && workspace, RLPYT_EINVAL, "rlpyt_policy_kl_loss_fwd_bwd: null pointer");
+  RL_CHECK_ARG(N == 0 || (logits && action && old_logp && advantage), RLPYT_EINVAL,
+               "rlpyt_policy_kl_loss_fwd_bwd: null pointer");
+  RL_CHECK_ARG((logp == nullptr) == (entropy == nullptr), RLPYT_EINVAL,
+               "rlpyt_policy_kl_loss_fwd_bwd: logp and entropy come together");
+  hipStream_t s = (hipStream_t)stream;
+  const LossPlan q = plan_of(N, V, element_size(dtype));
+  LossArgs p = {};
+  p.logits = logits, p.row_stride = row_stride, p.action = action, p.old_logp = old_logp, p.advantage = advantage;
+  p.ref_logp = ref_logp, p.valid = valid, p.grad = grad, p.logp = logp, p.entropy = entropy;
+  double* denom = (double*)workspace;
+  p.rows = (double*)((char*)workspace + 16);
+  p.denom = valid ? denom : nullptr;
+  p.parts = (float3*)((char*)workspace + parts_offset(q));
+  p.N = N, p.V = (int)V, p.part = q.part;
+  p.lo = clip_low, p.hi = clip_high, p.c_kl = kl_coeff, p.c_ent = entropy_coeff;
+  if (valid) RL_LAUNCH(loss_denom_kernel, dim3(1), dim3(1024), 0, s, valid, N, denom);
+  const int rc = run_all(dtype, p, q, s);
+  if (rc != RLPYT_OK) return rc;
+  RL_LAUNCH(loss_finish_kernel, dim3(1), dim3(1024), 0, s, p.rows, N ? q.partials : 0, p.denom, (double)N, kl_coeff,
+            entropy_coeff, scalars);
+  RL_LAUNCH_CHECK();
+  return RLPYT_OK;
+}
+
+extern "C" int rlpyt_action_logp(int dtype, const void* logits, int64_t row_stride, const int64_t* action,
+                                 int64_t N, int64_t V, float* logp, float* entropy, void* workspace,
+                                 rlpyt_stream_t stream) {
+  RL_CHECK_ARG(dtype >= F32 && dtype <= F16, RLPYT_EINVAL, "rlpyt_action_logp: unknown dtype %d", dtype);
+  RL_CHECK_ARG(N >= 0 && V > 0 && V <= (1 << 30), RLPYT_ESHAPE, "rlpyt_action_logp: N=%ld V=%ld out of range",
+               (long)N, (long)V);
+  if (N == 0) return RLPYT_OK;
+  RL_CHECK_ARG(logits && action && logp && entropy && workspace, RLPYT_EINVAL, "rlpyt_action_logp: null pointer");
+  const LossPlan q = plan_of(N, V, element_size(dtype));
+  LossArgs p = {};
+  p.logits = logits, p.row_stride = row_stride, p.action = action, p.logp = logp, p.entropy = entropy;
+  p.parts = (float3*)((char*)workspace + parts_offset(q));
+  p.N = N, p.V = (int)V, p.part = q.part;
+  return run_all(dtype, p, q, (hipStream_t)stream);
+}
+
+extern "C" int rlpyt_scale_unless_one(int dtype, void* x, int64_t n, const float* scale, rlpyt_stream_t stream) {
+  RL_CHECK_ARG(dtype >= F32 && dtype <= F16, RLPYT_EINVAL, "rlpyt_scale_unless_one: unknown dtype %d", dtype);
+  RL_CHECK_ARG(n >= 0 && n < ((int64_t)1 << 34), RLPYT_ESHAPE, "rlpyt_scale_unless_one: n=%ld out of range", (long)n);
+  if (n == 0) return RLPYT_OK;
+  RL_CHECK_ARG(x && scale, RLPYT_EINVAL, "rlpyt_scale_unless_one: null pointer");
+  RL_CHECK_ARG(RL_ALIGNED16(x), RLPYT_ESHAPE, "rlpyt_scale_unless_one: x must be 16-byte aligned");
+  hipStream_t s = (hipStream_t)stream;
+  const int per = 256 * (16 / element_size(dtype));
+  const dim3 grid((unsigned)ceil_div(n, per));
+  if (dtype == F32) RL_LAUNCH((loss_scale_kernel<float>), grid, dim3(256), 0, s, (float*)x, n, scale);
+  else if (dtype == BF16) RL_LAUNCH((loss_scale_kernel<__bf16>), grid, dim3(256), 0, s, (__bf16*)x, n, scale);
+  else RL_LAUNCH((loss_scale_kernel<_Float16>), grid, dim3(256), 0, s, (_Float16*)x, n, scale);
+  RL_LAUNCH_CHECK();
+  return RLPYT_OK;
+}

@@ -1764,3 +1764,10 @@ class DeviceSumTree:
         check(lib.rlpyt_sumtree_copy_tree(self._h, ptr(out), stream()),
               "rlpyt_sumtree_copy_tree")
         return out
+
+
+# --------------------------------------------------------------------------------------
+# long sequences, large action sets, matrix updates (ops_seq.py)
+# --------------------------------------------------------------------------------------
+from .ops_seq import (action_logp, gated_scan, gated_scan_step, orthogonalize,  # noqa: E402,F401
+                      policy_kl_loss)

@@ -211,3 +211,93 @@ class ClipAdam(torch.optim.Adam):
             return norm_out
         self._opt_called = True    # (torch's LR schedulers check that a step preceded theirs)
         return self._norm
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum whose update of every weight matrix is orthogonalised (``ops.orthogonalize``): its singular
+    values become about 1, so that no direction of the gradient's spectrum dominates a step::
+
+        buf <- momentum buf + (1 - momentum) g        u = g + momentum (buf - g) if nesterov else buf
+        W <- (1 - lr weight_decay) W - lr sqrt(max(1, m / n)) orthogonalize(u)
+
+    Parameters with two or more axes are taken as matrices ``[m, rest]`` (a convolution's filters are its rows); the others
+    (biases, gains) get Adam steps of ``lr * adam_lr_ratio``.  ``lr`` is a matrix' step per update: 0.02 is usual,
+    not Adam's 1e-3.
+
+    An algorithm takes it as ``OptimCls=Muon``; ``clip_and_step`` is what the algorithms here call.  All matrices of a step go
+    through the same few launches; float32, bfloat16 and float16 parameters on the device."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0., ns_steps=5,
+                 ns_coeffs=(3.4445, -4.7750, 2.0315), ns_eps=1e-7, adam_lr_ratio=0.05, adam_betas=(0.9, 0.999),
+                 adam_eps=1e-8):
+        if lr < 0. or not 0. <= momentum < 1. or weight_decay < 0. or adam_lr_ratio < 0.:
+            raise ValueError("Muon: lr, weight_decay, adam_lr_ratio >= 0 and 0 <= momentum < 1 are needed")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
+                                      ns_steps=ns_steps, ns_coeffs=tuple(ns_coeffs), ns_eps=ns_eps,
+                                      adam_lr_ratio=adam_lr_ratio, adam_betas=tuple(adam_betas), adam_eps=adam_eps))
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None]
+            self._matrix_step(group, [p for p in params if p.dim() >= 2])
+            self._vector_step(group, [p for p in params if p.dim() < 2])
+        return loss
+
+    def _matrix_step(self, group, params):
+        if not params:
+            return
+        from .ops import orthogonalize
+        beta, lr = group["momentum"], float(group["lr"])
+        grads = [p.grad for p in params]
+        for p in params:
+            if not self.state[p]:
+                self.state[p]["momentum_buffer"] = torch.zeros_like(p)
+        bufs = [self.state[p]["momentum_buffer"] for p in params]
+        torch._foreach_lerp_(bufs, grads, 1. - beta)
+        updates = torch._foreach_lerp(grads, bufs, beta) if group["nesterov"] else bufs
+        updates = orthogonalize([u.reshape(u.shape[0], -1) for u in updates], steps=group["ns_steps"],
+                                coeffs=group["ns_coeffs"], eps=group["ns_eps"])
+        if group["weight_decay"]:
+            torch._foreach_mul_(params, 1. - lr * group["weight_decay"])
+        for p, u in zip(params, updates):
+            scale = math.sqrt(max(1., u.shape[0] / max(1, u.shape[1])))
+            p.add_(u.view(p.shape), alpha=-lr * scale)
+
+    def _vector_step(self, group, params):
+        if not params:
+            return
+        b1, b2 = group["adam_betas"]
+        lr = float(group["lr"]) * group["adam_lr_ratio"]
+        grads = [p.grad for p in params]
+        for p in params:
+            if not self.state[p]:
+                self.state[p].update(step=0, exp_avg=torch.zeros_like(p), exp_avg_sq=torch.zeros_like(p))
+            self.state[p]["step"] += 1
+        avgs, squares = ([self.state[p][k] for p in params] for k in ("exp_avg", "exp_avg_sq"))
+        torch._foreach_lerp_(avgs, grads, 1. - b1)
+        torch._foreach_mul_(squares, b2)
+        torch._foreach_addcmul_(squares, grads, grads, 1. - b2)
+        if group["weight_decay"]:
+            torch._foreach_mul_(params, 1. - lr * group["weight_decay"])
+        for p, m, v in zip(params, avgs, squares):
+            n = self.state[p]["step"]
+            denom = (v / (1. - b2 ** n)).sqrt_().add_(group["adam_eps"])
+            p.addcdiv_(m, denom, value=-lr / (1. - b1 ** n))
+
+    @torch.no_grad()
+    def clip_and_step(self, max_norm, norm_out=None):
+        """``clip_grad_norm_(params, max_norm)`` + ``step()``; returns the gradient norm before clipping
+        (device scalar).  ``max_norm`` None or <= 0: no clipping.  ``norm_out``: as in ``ClipAdam``."""
+        params = [p for g in self.param_groups for p in g["params"] if p.grad is not None]
+        if not params:
+            norm = torch.zeros((), device=self.param_groups[0]["params"][0].device)
+        else:
+            bound = float(max_norm) if max_norm and max_norm > 0 else math.inf
+            norm = torch.nn.utils.clip_grad_norm_(params, bound)
+        self.step()
+        return ClipAdam._to_out(norm, norm_out)

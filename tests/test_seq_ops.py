@@ -1,0 +1,112 @@
+"""Refusals of the sequence operators (no GPU needed): wrong shapes, types and options raise before any device
+call, and the C entry points return error codes with a message."""
+import ctypes
+
+import pytest
+import torch
+
+from rlpyt_amd import _lib, ops
+from rlpyt_amd.optim import Muon
+
+z = torch.zeros
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ops.gated_scan(z(3, 2), z(3, 2)),                                       # not [T, B, D]
+    lambda: ops.gated_scan(z(3, 2, 4), z(3, 2, 5)),
+    lambda: ops.gated_scan(z(3, 2, 4), z(3, 2, 4).bfloat16()),                      # two types
+    lambda: ops.gated_scan(z(3, 2, 4).double(), z(3, 2, 4).double()),
+    lambda: ops.gated_scan(z(3, 2, 4), z(3, 2, 4), h0=z(4, 2)),
+    lambda: ops.gated_scan(z(3, 2, 4), z(3, 2, 4), h0=z(2, 4).long()),
+    lambda: ops.gated_scan(z(3, 2, 4), z(3, 2, 4), reset=z(2, 3).bool()),
+    lambda: ops.gated_scan(z(3, 2, 4), z(3, 2, 4), lengths=z(2)),                   # not whole numbers
+    lambda: ops.gated_scan(z(3, 2, 4), z(3, 2, 4), lengths=z(3).long()),
+    lambda: ops.gated_scan_step(z(2, 4), z(4, 2), z(2, 4)),
+    lambda: ops.gated_scan_step(z(2, 4), z(2, 4), z(2, 4).bfloat16()),              # the state is float32
+    lambda: ops.gated_scan_step(z(2, 4), z(2, 4), z(4, 2).t()),                     # and dense
+    lambda: ops.gated_scan_step(z(2, 4), z(2, 4), z(2, 4), reset=z(4).bool()),
+    lambda: ops.gated_scan_step(z(2, 4, requires_grad=True), z(2, 4), z(2, 4)),
+    lambda: ops.policy_kl_loss(z(3, 0), z(3).long(), z(3), z(3)),
+    lambda: ops.policy_kl_loss(z(3, 4).double(), z(3).long(), z(3), z(3)),
+    lambda: ops.policy_kl_loss(z(3, 4), z(3), z(3), z(3)),                          # action not whole
+    lambda: ops.policy_kl_loss(z(3, 4), z(4).long(), z(3), z(3)),
+    lambda: ops.policy_kl_loss(z(3, 4), z(3).long(), z(4), z(3)),
+    lambda: ops.policy_kl_loss(z(3, 4), z(3).long(), z(3), z(1)),
+    lambda: ops.policy_kl_loss(z(3, 4), z(3).long(), z(3), z(3), valid=z(3, 1)),
+    lambda: ops.policy_kl_loss(z(3, 4), z(3).long(), z(3), z(3), kl_coeff=0.1),     # no ref_logp
+    lambda: ops.policy_kl_loss(z(3, 4), z(3).long(), z(3), z(3), clip_low=1.5),
+    lambda: ops.policy_kl_loss(z(3, 4), z(3).long(), z(3), z(3), clip_high=-0.1),
+    lambda: ops.policy_kl_loss(z(3, 4), z(3).long(), z(3), z(3), clip_high=float("nan")),
+    lambda: ops.action_logp(z(3, 4), z(3)),
+    lambda: ops.action_logp(z(3, 4).long(), z(3).long()),
+    lambda: ops.orthogonalize(z(4)),
+    lambda: ops.orthogonalize([z(4, 4), z(4, 4).double()]),
+    lambda: ops.orthogonalize(z(4, 4), steps=0),
+    lambda: ops.orthogonalize(z(4, 4), steps=2.5),
+    lambda: ops.orthogonalize(z(4, 4), coeffs=(1., 2.)),
+    lambda: ops.orthogonalize(z(4, 4), eps=-1.),
+    lambda: Muon([z(3, 3, requires_grad=True)], lr=-1.),
+    lambda: Muon([z(3, 3, requires_grad=True)], momentum=1.),
+])
+def test_refused(call):
+    with pytest.raises(ValueError):
+        call()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="GPU present")
+def test_no_cpu_fallback():
+    for call in (lambda: ops.gated_scan(z(3, 2, 4), z(3, 2, 4)), lambda: ops.gated_scan_step(z(2, 4), z(2, 4), z(2, 4)),
+                 lambda: ops.policy_kl_loss(z(3, 4), z(3).long(), z(3), z(3)),
+                 lambda: ops.action_logp(z(3, 4), z(3).long()), lambda: ops.orthogonalize(z(4, 4))):
+        with pytest.raises(_lib.HipError):
+            call()
+
+
+def test_orthogonalize_of_nothing():
+    assert ops.orthogonalize([]) == []
+
+
+def test_entry_points_validate_without_a_gpu():
+    lib = _lib.lib
+    buf = (ctypes.c_float * 64)()
+    p = ctypes.cast(buf, ctypes.c_void_p)
+    fwd, bwd = lib.rlpyt_gated_scan_fwd, lib.rlpyt_gated_scan_bwd
+    # nothing to do
+    assert fwd(0, None, 0, 0, None, 0, 0, None, None, None, None, 0, 0, None, None, 0, 2, 4, None, None) == 0
+    assert bwd(0, None, 0, 0, None, 0, 0, None, 0, 0, None, None, None, None, None, 0, 0, None, 0, 0, None, 3, 0, 4,
+               None, None) == 0
+    # unknown type, sizes out of range, null pointers
+    assert fwd(3, p, 0, 0, p, 0, 0, None, None, None, p, 0, 0, None, None, 1, 1, 4, None, None) != 0
+    assert b"dtype" in lib.rlpyt_hip_last_error()
+    assert fwd(0, p, 0, 0, p, 0, 0, None, None, None, p, 0, 0, None, None, -1, 1, 4, None, None) != 0
+    assert fwd(0, p, 0, 0, p, 0, 0, None, None, None, p, 0, 0, None, None, 1, 1 << 20, 1 << 20, None, None) != 0
+    assert b"out of range" in lib.rlpyt_hip_last_error()
+    assert fwd(0, None, 0, 0, p, 0, 0, None, None, None, p, 0, 0, None, None, 1, 1, 4, None, None) != 0
+    assert b"null pointer" in lib.rlpyt_hip_last_error()
+    # a long sequence of few channels needs its workspace
+    assert lib.rlpyt_gated_scan_workspace_bytes(1 << 16, 1, 512) > 0
+    assert fwd(0, p, 0, 0, p, 0, 0, None, None, None, p, 0, 0, None, None, 1 << 16, 1, 512, None, None) != 0
+    assert b"workspace" in lib.rlpyt_hip_last_error()
+    assert lib.rlpyt_gated_scan_workspace_bytes(0, 1, 512) == 0
+    assert lib.rlpyt_gated_scan_state_rows(0) == 0 and lib.rlpyt_gated_scan_state_rows(1) == 1
+    assert lib.rlpyt_gated_scan_step(0, None, 0, None, 0, None, None, None, 0, 4, None) == 0
+    assert lib.rlpyt_gated_scan_step(0, None, 0, None, 0, None, None, None, 2, 4, None) != 0
+    loss = lib.rlpyt_policy_kl_loss_fwd_bwd
+    assert loss(0, p, 4, p, p, p, None, None, 2, 0, .2, .2, 0., 0., p, None, None, None, p, None) != 0
+    assert loss(0, None, 4, p, p, p, None, None, 2, 4, .2, .2, 0., 0., p, None, None, None, p, None) != 0
+    assert loss(0, p, 4, p, p, p, None, None, 2, 4, .2, .2, 0., 0., p, p, None, None, p, None) != 0
+    assert b"together" in lib.rlpyt_hip_last_error()
+    assert loss(0, p, 4, p, p, p, None, None, 2, 4, .2, .2, 0., 0., None, None, None, None, p, None) != 0
+    assert lib.rlpyt_action_logp(0, None, 4, None, 0, 4, None, None, None, None) == 0
+    assert lib.rlpyt_action_logp(0, None, 4, None, 2, 4, None, None, None, None) != 0
+    assert lib.rlpyt_scale_unless_one(0, None, 0, None, None) == 0
+    assert lib.rlpyt_scale_unless_one(0, None, 4, None, None) != 0
+    one = (ctypes.c_void_p * 1)(p.value)
+    side, big = (ctypes.c_int64 * 1)(4), (ctypes.c_int64 * 1)(1 << 20)
+    orth = lib.rlpyt_orthogonalize
+    assert orth(0, None, None, None, None, None, 0, 5, 1., 0., 0., 0., None, None) == 0
+    assert orth(0, one, side, one, big, side, 1, 5, 1., 0., 0., 0., p, None) != 0
+    assert orth(0, one, side, one, side, side, 1, 5, 1., 0., 0., 0., None, None) != 0
+    assert orth(0, one, side, one, side, side, 1, 5, 9., 0., 0., 0., p, None) != 0     # leaves f16's range
+    assert b"range of the stored factors" in lib.rlpyt_hip_last_error()
+    assert orth(0, one, side, one, side, side, 1, 5, float("nan"), 0., 0., 0., p, None) != 0
