@@ -390,7 +390,8 @@ __global__ __launch_bounds__(1024) void loss_denom_kernel(const float* __restric
 
 __global__ __launch_bounds__(1024) void loss_finish_kernel(const double* __restrict__ rows, int64_t n,
                                                            const double* __restrict__ denom, double N, double c_kl,
-                                                           double c_ent, float* __restrict__ scalars) {
+                                                           double c_ent, float* __restrict__ loss,
+                                                           float* __restrict__ scalars) {
   __shared__ double scratch[4 * 16];
   double v[4] = {0.0, 0.0, 0.0, 0.0};
   for (int64_t i = threadIdx.x; i < n; i += 1024)
@@ -401,11 +402,11 @@ __global__ __launch_bounds__(1024) void loss_finish_kernel(const double* __restr
   const double d = denom ? *denom : N;
   const double inv = d > 0.0 ? 1.0 / d : 0.0;   // nothing valid: a loss of 0
   for (int k = 0; k < 4; ++k) v[k] *= inv;
-  scalars[0] = (float)(v[0] + c_kl * v[1] - c_ent * v[2]);
+  *loss = scalars[0] = (float)(v[0] + c_kl * v[1] - c_ent * v[2]);
   for (int k = 0; k < 4; ++k) scalars[1 + k] = (float)v[k];
 }
 
-// grad *= *scale, in place; nothing is read or written where *scale is 1.
+// grad *= *scale, in place; nothing is read or written where *scale is 1 (hence a grid that the chip holds at once).
 template <typename E>
 __global__ __launch_bounds__(256) void loss_scale_kernel(E* __restrict__ g, int64_t n,
                                                          const float* __restrict__ scale) {
@@ -413,15 +414,15 @@ __global__ __launch_bounds__(256) void loss_scale_kernel(E* __restrict__ g, int6
   constexpr int n16 = Row16<E>::n;
   const float f = *scale;
   if (f == 1.f) return;
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * n16;
-  if (i >= n) return;
-  if (i + n16 <= n) {
-    vec v = *reinterpret_cast<const vec*>(g + i);
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * n16; i < n; i += (int64_t)gridDim.x * 256 * n16) {
+    if (i + n16 <= n) {
+      vec v = *reinterpret_cast<const vec*>(g + i);
 #pragma unroll
-    for (int k = 0; k < n16; ++k) v[k] = (E)((float)v[k] * f);
-    *reinterpret_cast<vec*>(g + i) = v;
-  } else {
-    for (int64_t k = i; k < n; ++k) g[k] = (E)((float)g[k] * f);
+      for (int k = 0; k < n16; ++k) v[k] = (E)((float)v[k] * f);
+      *reinterpret_cast<vec*>(g + i) = v;
+    } else {
+      for (int64_t k = i; k < n; ++k) g[k] = (E)((float)g[k] * f);
+    }
   }
 }
 
@@ -517,21 +518,19 @@ extern "C" int rlpyt_policy_kl_loss_fwd_bwd(int dtype, const void* logits, int64
                                             const int64_t* action, const float* old_logp,
                                             const float* advantage, const float* ref_logp, const float* valid,
                                             int64_t N, int64_t V, double clip_low, double clip_high,
-                                            double kl_coeff, double entropy_coeff, float* scalars, float* logp,
-                                            float* entropy, void* grad, void* workspace, rlpyt_stream_t stream) {
+                                            double kl_coeff, double entropy_coeff, float* loss, float* scalars,
+                                            void* grad, void* workspace, rlpyt_stream_t stream) {
   RL_CHECK_ARG(dtype >= F32 && dtype <= F16, RLPYT_EINVAL, "rlpyt_policy_kl_loss_fwd_bwd: unknown dtype %d", dtype);
   RL_CHECK_ARG(N >= 0 && V > 0 && V <= (1 << 30), RLPYT_ESHAPE,
                "rlpyt_policy_kl_loss_fwd_bwd: N=%ld V=%ld out of range", (long)N, (long)V);
-  RL_CHECK_ARG(scalars && workspace, RLPYT_EINVAL, "rlpyt_policy_kl_loss_fwd_bwd: null pointer");
+  RL_CHECK_ARG(loss && scalars && workspace, RLPYT_EINVAL, "rlpyt_policy_kl_loss_fwd_bwd: null pointer");
   RL_CHECK_ARG(N == 0 || (logits && action && old_logp && advantage), RLPYT_EINVAL,
                "rlpyt_policy_kl_loss_fwd_bwd: null pointer");
-  RL_CHECK_ARG((logp == nullptr) == (entropy == nullptr), RLPYT_EINVAL,
-               "rlpyt_policy_kl_loss_fwd_bwd: logp and entropy come together");
   hipStream_t s = (hipStream_t)stream;
   const LossPlan q = plan_of(N, V, element_size(dtype));
   LossArgs p = {};
   p.logits = logits, p.row_stride = row_stride, p.action = action, p.old_logp = old_logp, p.advantage = advantage;
-  p.ref_logp = ref_logp, p.valid = valid, p.grad = grad, p.logp = logp, p.entropy = entropy;
+  p.ref_logp = ref_logp, p.valid = valid, p.grad = grad;
   double* denom = (double*)workspace;
   p.rows = (double*)((char*)workspace + 16);
   p.denom = valid ? denom : nullptr;
@@ -542,7 +541,7 @@ extern "C" int rlpyt_policy_kl_loss_fwd_bwd(int dtype, const void* logits, int64
   const int rc = run_all(dtype, p, q, s);
   if (rc != RLPYT_OK) return rc;
   RL_LAUNCH(loss_finish_kernel, dim3(1), dim3(1024), 0, s, p.rows, N ? q.partials : 0, p.denom, (double)N, kl_coeff,
-            entropy_coeff, scalars);
+            entropy_coeff, loss, scalars);
   RL_LAUNCH_CHECK();
   return RLPYT_OK;
 }
@@ -565,13 +564,13 @@ extern "C" int rlpyt_action_logp(int dtype, const void* logits, int64_t row_stri
 
 extern "C" int rlpyt_scale_unless_one(int dtype, void* x, int64_t n, const float* scale, rlpyt_stream_t stream) {
   RL_CHECK_ARG(dtype >= F32 && dtype <= F16, RLPYT_EINVAL, "rlpyt_scale_unless_one: unknown dtype %d", dtype);
-  RL_CHECK_ARG(n >= 0 && n < ((int64_t)1 << 34), RLPYT_ESHAPE, "rlpyt_scale_unless_one: n=%ld out of range", (long)n);
+  RL_CHECK_ARG(n >= 0, RLPYT_ESHAPE, "rlpyt_scale_unless_one: n=%ld out of range", (long)n);
   if (n == 0) return RLPYT_OK;
   RL_CHECK_ARG(x && scale, RLPYT_EINVAL, "rlpyt_scale_unless_one: null pointer");
   RL_CHECK_ARG(RL_ALIGNED16(x), RLPYT_ESHAPE, "rlpyt_scale_unless_one: x must be 16-byte aligned");
   hipStream_t s = (hipStream_t)stream;
   const int per = 256 * (16 / element_size(dtype));
-  const dim3 grid((unsigned)ceil_div(n, per));
+  const dim3 grid((unsigned)std::min<int64_t>(2048, ceil_div(n, per)));
   if (dtype == F32) RL_LAUNCH((loss_scale_kernel<float>), grid, dim3(256), 0, s, (float*)x, n, scale);
   else if (dtype == BF16) RL_LAUNCH((loss_scale_kernel<__bf16>), grid, dim3(256), 0, s, (__bf16*)x, n, scale);
   else RL_LAUNCH((loss_scale_kernel<_Float16>), grid, dim3(256), 0, s, (_Float16*)x, n, scale);

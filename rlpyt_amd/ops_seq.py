@@ -16,49 +16,56 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .utils import ktimer
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _FLOATS = (torch.float32, torch.float64, torch.bfloat16, torch.float16)
+_BYTES = (torch.bool, torch.uint8)
+# (torch.cuda.current_stream() builds a Stream object, 1 - 3 us a call; small calls here take 10)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _need(cond, text):
-    if not cond:
-        raise ValueError(text)
+def _refuse(text):
+    raise ValueError(text)
 
 
 def _need_device(name, first, *others):
-    _lib.require_gpu()
-    _need(first.is_cuda, f"{name}: tensors on the device are needed, got {first.device}")
+    if not first.is_cuda:
+        _lib.require_gpu()
+        _refuse(f"{name}: tensors on the device are needed, got {first.device}")
+    device = first.device
     for t in others:
-        _need(t is None or t.device == first.device,
-              f"{name}: tensors on one device are needed, got {first.device} and {getattr(t, 'device', None)}")
+        if t is not None and t.device != device:
+            _refuse(f"{name}: tensors on one device are needed, got {device} and {t.device}")
 
 
 def _p(t):
     return None if t is None else t.data_ptr()
 
 
-class _on:
-    """The device of ``t`` as the current one; ``as`` gives its current stream."""
-    __slots__ = ("index", "before")
-
-    def __init__(self, t):
-        self.index = t.device.index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+def _launch(index, fn, *args):
+    """``fn(*args, stream)`` on device ``index`` and its current stream."""
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc, fn.__name__)
 
 
-def _bytes(n, like):
-    return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None
+def _bytes(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def _backward(fast):
+    """A backward pass that is not differentiable itself: the check costs 8 us, and is needed only where a graph
+    of the backward pass is built (gradients are enabled inside it then)."""
+    checked = torch.autograd.function.once_differentiable(fast)
+
+    def backward(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else fast(ctx, *grads)
+
+    return staticmethod(backward)
 
 
 # --------------------------------------------------------------------------------------
@@ -71,6 +78,8 @@ def _unit_rows(t):
 
 def _like_rows(x):
     """An empty ``[T, B, D]`` whose rows lie in memory in the order of ``x``'s: time or batch first."""
+    if x.is_contiguous():
+        return torch.empty_like(x)
     T, B, D = x.shape
     if T > 1 and B > 1 and x.stride(1) > x.stride(0):
         return torch.empty((B, T, D), dtype=x.dtype, device=x.device).transpose(0, 1)
@@ -79,51 +88,64 @@ def _like_rows(x):
 
 def _scan_forward(x, gate, h0, reset, lengths, keep):
     T, B, D = x.shape
+    device = x.device
     h = _like_rows(x)
-    hn = torch.empty((B, D), dtype=torch.float32, device=x.device)
-    states = (torch.empty((lib.rlpyt_gated_scan_state_rows(T), B, D), dtype=torch.float32, device=x.device)
+    hn = torch.empty((B, D), dtype=torch.float32, device=device)
+    states = (torch.empty((lib.rlpyt_gated_scan_state_rows(T), B, D), dtype=torch.float32, device=device)
               if keep else None)
-    ws = _bytes(lib.rlpyt_gated_scan_workspace_bytes(T, B, D), x)
-    with _on(x) as stream, ktimer.region("gated_scan", 3 * x.numel() * x.element_size()):
-        check(lib.rlpyt_gated_scan_fwd(
-            _DTYPES[x.dtype], x.data_ptr(), x.stride(0), x.stride(1), gate.data_ptr(), gate.stride(0),
-            gate.stride(1), _p(h0), _p(reset), _p(lengths), h.data_ptr(), h.stride(0), h.stride(1),
-            hn.data_ptr(), _p(states), T, B, D, _p(ws), stream), "rlpyt_gated_scan_fwd")
+    ws = _bytes(lib.rlpyt_gated_scan_workspace_bytes(T, B, D), device)
+    _launch(device.index, lib.rlpyt_gated_scan_fwd, _DTYPES[x.dtype], x.data_ptr(), *x.stride()[:2],
+            gate.data_ptr(), *gate.stride()[:2], _p(h0), _p(reset), _p(lengths), h.data_ptr(), *h.stride()[:2],
+            hn.data_ptr(), _p(states), T, B, D, _p(ws))
     return h, hn, states
+
+
+def _scan_backward(ctx, dh, dhn):
+    if dh is None and dhn is None:
+        return None, None, None, None, None
+    x, gate, reset, lengths, states = ctx.saved_tensors
+    T, B, D = x.shape
+    dtype, device = x.dtype, x.device
+    if dh is None:
+        dh = torch.zeros(D, dtype=dtype, device=device).expand(T, B, D)
+    elif dh.dtype != dtype or (dh.stride(-1) != 1 and D != 1):
+        dh = dh.to(dtype).contiguous()
+    if dhn is not None and not (dhn.dtype == torch.float32 and dhn.is_contiguous()):
+        dhn = dhn.to(torch.float32).contiguous()
+    dx, dgate = _like_rows(x), _like_rows(x)
+    dh0 = torch.empty((B, D), dtype=torch.float32, device=device) if ctx.needs_input_grad[2] else None
+    ws = _bytes(ctx.ws_bytes, device)
+    strides = dx.stride()[:2]
+    _launch(device.index, lib.rlpyt_gated_scan_bwd, _DTYPES[dtype], x.data_ptr(), *x.stride()[:2],
+            gate.data_ptr(), *gate.stride()[:2], dh.data_ptr(), *dh.stride()[:2], _p(dhn), _p(reset), _p(lengths),
+            states.data_ptr(), dx.data_ptr(), *strides, dgate.data_ptr(), *strides, _p(dh0), T, B, D, _p(ws))
+    if dh0 is not None and ctx.h0_dtype != torch.float32:
+        dh0 = dh0.to(ctx.h0_dtype)
+    return dx, dgate, dh0, None, None
 
 
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, h0, reset, lengths):
-        h0f = None if h0 is None else h0.detach().to(torch.float32).contiguous()
-        h, hn, states = _scan_forward(x, gate, h0f, reset, lengths, True)
+        h0_dtype = None if h0 is None else h0.dtype
+        h, hn, states = _scan_forward(x, gate, _state32(h0), reset, lengths, True)
         ctx.save_for_backward(x, gate, reset, lengths, states)
-        ctx.h0_dtype = None if h0 is None else h0.dtype
+        ctx.h0_dtype = h0_dtype
+        ctx.ws_bytes = lib.rlpyt_gated_scan_workspace_bytes(*x.shape)
         ctx.set_materialize_grads(False)
         return h, hn
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dh, dhn):
-        x, gate, reset, lengths, states = ctx.saved_tensors
-        if dh is None and dhn is None:
-            return None, None, None, None, None
-        T, B, D = x.shape
-        if dh is None:
-            dh = torch.zeros(D, dtype=x.dtype, device=x.device).expand(T, B, D)
-        dh = _unit_rows(dh.to(x.dtype))
-        dhn = None if dhn is None else dhn.to(torch.float32).contiguous()
-        dx, dgate = _like_rows(x), _like_rows(x)
-        dh0 = (torch.empty((B, D), dtype=torch.float32, device=x.device)
-               if ctx.h0_dtype is not None and ctx.needs_input_grad[2] else None)
-        ws = _bytes(lib.rlpyt_gated_scan_workspace_bytes(T, B, D), x)
-        with _on(x) as stream, ktimer.region("gated_scan_bwd", 5 * x.numel() * x.element_size()):
-            check(lib.rlpyt_gated_scan_bwd(
-                _DTYPES[x.dtype], x.data_ptr(), x.stride(0), x.stride(1), gate.data_ptr(), gate.stride(0),
-                gate.stride(1), dh.data_ptr(), dh.stride(0), dh.stride(1), _p(dhn), _p(reset), _p(lengths),
-                states.data_ptr(), dx.data_ptr(), dx.stride(0), dx.stride(1), dgate.data_ptr(), dgate.stride(0),
-                dgate.stride(1), _p(dh0), T, B, D, _p(ws), stream), "rlpyt_gated_scan_bwd")
-        return dx, dgate, None if dh0 is None else dh0.to(ctx.h0_dtype), None, None
+    backward = _backward(_scan_backward)
+
+
+def _state32(h0):
+    if h0 is None or (h0.dtype == torch.float32 and h0.is_contiguous()):
+        return h0
+    return h0.detach().to(torch.float32).contiguous()
+
+
+def _reset_bytes(reset):
+    return (reset if reset.dtype in _BYTES else reset != 0).contiguous()
 
 
 def gated_scan(x, gate, h0=None, reset=None, lengths=None):
@@ -135,63 +157,73 @@ def gated_scan(x, gate, h0=None, reset=None, lengths=None):
     Differentiable w.r.t. ``x``, ``gate`` and ``h0`` (once).
 
     ``x, gate``: float32, bfloat16 or float16, any strides along time and batch (a ``[B, T, D]`` tensor goes
-    in as its ``transpose(0, 1)``, the halves of one projection as its ``chunk(2, -1)``).
-    ``h0 [B, D]``: the state before the first step (None: 0); a bfloat16 or float16 one is widened.
+    in as its ``transpose(0, 1)``, the halves of one projection as its ``chunk(2, -1)``); up to 2^28 channels ``B D``.
+    ``h0 [B, D]``: the state before the first step (None: 0); other floating types are converted to float32.
     ``reset [T, B]`` (bool, uint8 or nonzero float, as ``done``): the state is cleared BEFORE step t, whatever it
     held.  ``lengths [B]`` (integers, clamped to 0 .. T): steps from ``lengths[b]`` on are not part of sequence b:
     their ``x``, ``gate`` and incoming gradients are not used, their ``h`` and gradients are 0, and ``hn`` is
     the state behind the last step that is (``h0`` for a length of 0).
 
     States, sums and products are float32, also between the steps of a bfloat16 sequence."""
-    _need(x.dim() == 3 and x.shape == gate.shape,
-          f"gated_scan: x and gate [T, B, D] are needed, got {tuple(x.shape)} and {tuple(gate.shape)}")
+    if x.dim() != 3 or x.shape != gate.shape:
+        _refuse(f"gated_scan: x and gate [T, B, D] are needed, got {tuple(x.shape)} and {tuple(gate.shape)}")
     T, B, D = x.shape
-    _need(x.dtype in _DTYPES and gate.dtype == x.dtype,
-          f"gated_scan: x and gate of one type, float32, bfloat16 or float16, are needed, got {x.dtype} and {gate.dtype}")
-    _need(h0 is None or (h0.shape == (B, D) and h0.dtype in _FLOATS),
-          "gated_scan: h0 has to be [B, D] and floating")
-    _need(reset is None or (reset.shape == (T, B) and not reset.is_complex()), "gated_scan: reset has to be [T, B]")
-    _need(lengths is None or (lengths.shape == (B,) and lengths.dtype in (torch.int32, torch.int64)),
-          "gated_scan: lengths has to be [B], int32 or int64")
+    if x.dtype not in _DTYPES or gate.dtype != x.dtype:
+        _refuse(f"gated_scan: x and gate of one type, float32, bfloat16 or float16, are needed, got {x.dtype} "
+                f"and {gate.dtype}")
+    if h0 is not None and (h0.shape != (B, D) or h0.dtype not in _FLOATS):
+        _refuse(f"gated_scan: h0 has to be [B, D] and floating, got {tuple(h0.shape)} {h0.dtype}")
+    if reset is not None and (reset.shape != (T, B) or reset.is_complex()):
+        _refuse(f"gated_scan: reset has to be [T, B], got {tuple(reset.shape)}")
+    if lengths is not None and (lengths.shape != (B,) or lengths.dtype not in (torch.int32, torch.int64)):
+        _refuse(f"gated_scan: lengths has to be [B], int32 or int64, got {tuple(lengths.shape)} {lengths.dtype}")
     _need_device("gated_scan", x, gate, h0, reset, lengths)
     if x.numel() == 0:
         hn = torch.zeros((B, D), dtype=torch.float32, device=x.device) if h0 is None else h0.float()
         return x + gate, hn + 0.
     if reset is not None:
-        reset = (reset if reset.dtype in (torch.bool, torch.uint8) else reset != 0).contiguous().view(torch.uint8)
+        reset = _reset_bytes(reset)
     if lengths is not None:
         lengths = lengths.to(torch.int64).contiguous()
-    x, gate = _unit_rows(x), _unit_rows(gate)
+    if D != 1:
+        if x.stride(-1) != 1:
+            x = x.contiguous()
+        if gate.stride(-1) != 1:
+            gate = gate.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (h0 is not None and h0.requires_grad)):
         return _GatedScan.apply(x, gate, h0, reset, lengths)
-    h0 = None if h0 is None else h0.detach().to(torch.float32).contiguous()
-    return _scan_forward(x.detach(), gate.detach(), h0, reset, lengths, False)[:2]
+    return _scan_forward(x, gate, _state32(h0), reset, lengths, False)[:2]
 
 
 def gated_scan_step(x, gate, state, reset=None):
     """One step of ``gated_scan`` for a sampler or a server: ``x, gate [B, D]``, ``state [B, D]`` float32,
     dense, UPDATED IN PLACE; ``reset [B]`` clears a row's state first.  Returns the new state in the type of
     ``x``.  One launch; not differentiable."""
-    _need(x.dim() == 2 and x.shape == gate.shape,
-          f"gated_scan_step: x and gate [B, D] are needed, got {tuple(x.shape)} and {tuple(gate.shape)}")
-    _need(x.dtype in _DTYPES and gate.dtype == x.dtype,
-          f"gated_scan_step: x and gate of one type, float32, bfloat16 or float16, are needed, got {x.dtype} and {gate.dtype}")
-    _need(state.shape == x.shape and state.dtype == torch.float32 and state.is_contiguous(),
-          "gated_scan_step: state has to be a dense float32 [B, D]")
-    _need(reset is None or reset.shape == x.shape[:1], "gated_scan_step: reset has to be [B]")
-    _need(not (torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad)),
-          "gated_scan_step: not differentiable; call gated_scan, or this under torch.no_grad()")
+    shape = x.shape
+    if len(shape) != 2 or gate.shape != shape:
+        _refuse(f"gated_scan_step: x and gate [B, D] are needed, got {tuple(shape)} and {tuple(gate.shape)}")
+    if x.dtype not in _DTYPES or gate.dtype != x.dtype:
+        _refuse(f"gated_scan_step: x and gate of one type, float32, bfloat16 or float16, are needed, got {x.dtype} "
+                f"and {gate.dtype}")
+    if state.shape != shape or state.dtype != torch.float32 or not state.is_contiguous():
+        _refuse("gated_scan_step: state has to be a dense float32 [B, D]")
+    if reset is not None and reset.shape != shape[:1]:
+        _refuse(f"gated_scan_step: reset has to be [B], got {tuple(reset.shape)}")
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad):
+        _refuse("gated_scan_step: not differentiable; call gated_scan, or this under torch.no_grad()")
     _need_device("gated_scan_step", x, gate, state, reset)
-    if reset is not None:
-        reset = (reset if reset.dtype in (torch.bool, torch.uint8) else reset != 0).contiguous()
-    x, gate = _unit_rows(x), _unit_rows(gate)
-    B, D = x.shape
-    y = torch.empty((B, D), dtype=x.dtype, device=x.device)
-    with _on(x) as stream:
-        check(lib.rlpyt_gated_scan_step(_DTYPES[x.dtype], x.data_ptr(), x.stride(0), gate.data_ptr(),
-                                        gate.stride(0), _p(reset), state.data_ptr(), y.data_ptr(), B, D, stream),
-              "rlpyt_gated_scan_step")
-    torch.autograd.graph.increment_version([state])   # written through a raw pointer
+    if reset is not None and not (reset.dtype in _BYTES and reset.is_contiguous()):
+        reset = _reset_bytes(reset)
+    B, D = shape
+    if D != 1:
+        if x.stride(-1) != 1:
+            x = x.contiguous()
+        if gate.stride(-1) != 1:
+            gate = gate.contiguous()
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    _launch(x.get_device(), lib.rlpyt_gated_scan_step, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), gate.data_ptr(),
+            gate.stride(0), _p(reset), state.data_ptr(), y.data_ptr(), B, D)
+    torch.autograd.graph.increment_version(state)   # written through a raw pointer
     return y
 
 
@@ -199,50 +231,64 @@ def gated_scan_step(x, gate, state, reset=None):
 # clipped policy loss with a KL term, on logits
 # --------------------------------------------------------------------------------------
 def _logit_rows(name, logits, action):
-    _need(logits.dim() >= 1 and logits.shape[-1] > 0 and logits.dtype in _DTYPES,
-          f"{name}: logits [..., V] in float32, bfloat16 or float16 are needed, got {tuple(logits.shape)} {logits.dtype}")
-    _need(action.shape == logits.shape[:-1] and not action.is_floating_point() and action.dtype != torch.bool,
-          f"{name}: one whole action per row of logits is needed, got {tuple(action.shape)} {action.dtype}")
+    """The rows ``[N, V]`` of ``logits [..., V]`` with unit stride along V (a view where the strides allow one), and the
+    flat int64 actions."""
+    if logits.dim() < 1 or logits.shape[-1] == 0 or logits.dtype not in _DTYPES:
+        _refuse(f"{name}: logits [..., V] in float32, bfloat16 or float16 are needed, got {tuple(logits.shape)} "
+                f"{logits.dtype}")
+    if action.shape != logits.shape[:-1] or action.is_floating_point() or action.dtype == torch.bool:
+        _refuse(f"{name}: one whole action per row of logits is needed, got {tuple(action.shape)} {action.dtype}")
+    _need_device(name, logits, action)
+    rows = logits.detach()
+    if rows.dim() != 2:
+        rows = rows.reshape(-1, rows.shape[-1])
+    if rows.stride(-1) != 1 and rows.shape[-1] != 1:
+        rows = rows.contiguous()
+    if action.dtype != torch.int64 or not action.is_contiguous():
+        action = action.to(torch.int64).contiguous()
+    return rows, action
 
 
-def _flat_rows(logits):
-    """``[..., V]`` -> ``[N, V]`` with unit stride along V (a view where the strides allow one)."""
-    return _unit_rows(logits.detach().reshape(-1, logits.shape[-1]))
+def _numbers(t):
+    """Dense float32, in the order of the rows."""
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().to(torch.float32).contiguous()
+
+
+def _loss_forward(rows, numbers, coeffs, want_grad):
+    """One pass over ``rows [N, V]`` -> loss, scalars [5], gradient [N, V] or None."""
+    N, V = rows.shape
+    code, device = _DTYPES[rows.dtype], rows.device
+    scalars = torch.empty(5, dtype=torch.float32, device=device)
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    grad = torch.empty((N, V), dtype=rows.dtype, device=device) if want_grad else None
+    ws = _bytes(lib.rlpyt_policy_loss_workspace_bytes(code, N, V), device)
+    _launch(device.index, lib.rlpyt_policy_kl_loss_fwd_bwd, code, rows.data_ptr(), rows.stride(0),
+            *(_p(t) for t in numbers), N, V, *coeffs, loss.data_ptr(), scalars.data_ptr(), _p(grad), ws.data_ptr())
+    return loss, scalars, grad
+
+
+def _loss_backward(ctx, g_loss, _g_scalars):
+    grad, ctx.grad = ctx.grad, None
+    if grad is None:
+        raise RuntimeError("policy_kl_loss: its gradient went out with the first backward pass (it is scaled in place); "
+                           "run the loss again")
+    if not _is_unit_seed(g_loss):
+        _launch(grad.get_device(), lib.rlpyt_scale_unless_one, _DTYPES[grad.dtype], grad.data_ptr(), grad.numel(),
+                g_loss.data_ptr())
+    return (grad if ctx.shape is None else grad.reshape(ctx.shape)), None, None, None
 
 
 class _PolicyKlLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, action, old_logp, advantage, ref_logp, valid, clip_low, clip_high, kl_coeff,
-                entropy_coeff, needs_grad):
-        rows = _flat_rows(logits)
-        N, V = rows.shape
-        code = _DTYPES[rows.dtype]
-        scalars = torch.empty(5, dtype=torch.float32, device=rows.device)
-        grad = torch.empty((N, V), dtype=rows.dtype, device=rows.device) if needs_grad else None
-        ws = _bytes(lib.rlpyt_policy_loss_workspace_bytes(code, N, V), rows)
-        with _on(rows) as stream, ktimer.region("policy_kl_loss", (1 + needs_grad) * rows.numel() * rows.element_size()):
-            check(lib.rlpyt_policy_kl_loss_fwd_bwd(
-                code, rows.data_ptr(), rows.stride(0), action.data_ptr(), old_logp.data_ptr(),
-                advantage.data_ptr(), _p(ref_logp), _p(valid), N, V, clip_low, clip_high, kl_coeff,
-                entropy_coeff, scalars.data_ptr(), None, None, _p(grad), ws.data_ptr(), stream),
-                "rlpyt_policy_kl_loss_fwd_bwd")
-        ctx.grad, ctx.shape = grad, logits.shape
+    def forward(ctx, logits, rows, numbers, coeffs):
+        loss, scalars, grad = _loss_forward(rows, numbers, coeffs, True)
+        ctx.grad, ctx.shape = grad, None if logits.dim() == 2 else logits.shape
         ctx.mark_non_differentiable(scalars)
-        return scalars[0], scalars
+        return loss, scalars
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_loss, _g_scalars):
-        grad, ctx.grad = ctx.grad, None
-        if grad is None:
-            raise RuntimeError("policy_kl_loss: its gradient went out with the first backward pass (it is scaled in "
-                               "place); run the loss again")
-        from .ops import _is_unit_seed
-        if not _is_unit_seed(g_loss):
-            with _on(grad) as stream:
-                check(lib.rlpyt_scale_unless_one(_DTYPES[grad.dtype], grad.data_ptr(), grad.numel(),
-                                                 g_loss.float().data_ptr(), stream), "rlpyt_scale_unless_one")
-        return (grad.reshape(ctx.shape),) + (None,) * 10
+    backward = _backward(_loss_backward)
 
 
 def policy_kl_loss(logits, action, old_logp, advantage, ref_logp=None, valid=None, clip_low=0.2, clip_high=0.2,
@@ -255,7 +301,7 @@ def policy_kl_loss(logits, action, old_logp, advantage, ref_logp=None, valid=Non
 
     ``logits [..., V]`` float32, bfloat16 or float16, any row stride; ``action [...]`` whole numbers;
     ``old_logp, advantage, ref_logp [...]`` (the log-probabilities as ``action_logp`` gives them) and ``valid
-    [...]`` (weights, or a mask) are taken as float32.  ``mean_valid`` divides by the sum of ``valid``.
+    [...]`` (weights, or a mask) are taken as float32 and as constants.  ``mean_valid`` divides by the sum of ``valid``.
 
     Returns ``(loss, scalars)``: ``loss`` is differentiable w.r.t. ``logits`` (one backward pass a call: the
     gradient comes out of the forward pass, is scaled in place and handed on), ``scalars = [loss, pi_loss, kl,
@@ -265,42 +311,39 @@ def policy_kl_loss(logits, action, old_logp, advantage, ref_logp=None, valid=Non
     gradient, also where their action is out of range; nothing valid gives a loss of 0.  A row that allows
     no action adds 0 and has a zero gradient, but counts in the mean.  In a valid row an action outside 0 .. V-1 or a NaN
     logit makes the loss NaN; with a KL term, so does the gradient of an action that is not allowed (its kl is infinite)."""
-    _logit_rows("policy_kl_loss", logits, action)
     lead = logits.shape[:-1]
     for name, t in (("old_logp", old_logp), ("advantage", advantage), ("ref_logp", ref_logp), ("valid", valid)):
-        _need(t is None and name in ("ref_logp", "valid") or t is not None and t.shape == lead and not t.is_complex(),
-              f"policy_kl_loss: {name} has to be {tuple(lead)}, one number per row of logits")
-    _need(0. <= clip_low <= 1. and clip_high >= 0., "policy_kl_loss: 0 <= clip_low <= 1 and 0 <= clip_high are needed")
-    _need(ref_logp is not None or kl_coeff == 0., "policy_kl_loss: kl_coeff needs ref_logp")
-    _need_device("policy_kl_loss", logits, action, old_logp, advantage, ref_logp, valid)
-
-    def flat(t):
-        return None if t is None else t.detach().to(torch.float32).reshape(-1).contiguous()
-
-    action = action.reshape(-1).to(torch.int64).contiguous()
-    needs_grad = torch.is_grad_enabled() and logits.requires_grad
-    return _PolicyKlLoss.apply(logits, action, flat(old_logp), flat(advantage), flat(ref_logp), flat(valid),
-                               float(clip_low), float(clip_high), float(kl_coeff), float(entropy_coeff), needs_grad)
+        if t is None and name in ("ref_logp", "valid"):
+            continue
+        if t.shape != lead or t.is_complex():
+            _refuse(f"policy_kl_loss: {name} has to be {tuple(lead)}, one number per row of logits, got {tuple(t.shape)}")
+    if not (0. <= clip_low <= 1. and clip_high >= 0.):
+        _refuse("policy_kl_loss: 0 <= clip_low <= 1 and 0 <= clip_high are needed")
+    if ref_logp is None and kl_coeff != 0.:
+        _refuse("policy_kl_loss: kl_coeff needs ref_logp")
+    rows, action = _logit_rows("policy_kl_loss", logits, action)
+    _need_device("policy_kl_loss", rows, old_logp, advantage, ref_logp, valid)
+    numbers = (action, _numbers(old_logp), _numbers(advantage), _numbers(ref_logp), _numbers(valid))
+    coeffs = (float(clip_low), float(clip_high), float(kl_coeff), float(entropy_coeff))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _PolicyKlLoss.apply(logits, rows, numbers, coeffs)
+    return _loss_forward(rows, numbers, coeffs, False)[:2]
 
 
 def action_logp(logits, action):
     """``(log softmax(logits)[action], entropy)``, float32, of every row of ``logits [..., V]`` (float32,
     bfloat16 or float16): what ``policy_kl_loss`` takes as ``old_logp`` and ``ref_logp``.  Reads the logits once; not
     differentiable.  A row of -inf only gives ``(-inf, 0)``, an action outside 0 .. V-1 NaN."""
-    _logit_rows("action_logp", logits, action)
-    _need_device("action_logp", logits, action)
-    rows = _flat_rows(logits)
+    rows, action = _logit_rows("action_logp", logits, action)
     N, V = rows.shape
-    action = action.reshape(-1).to(torch.int64).contiguous()
-    code = _DTYPES[rows.dtype]
-    out = torch.empty((2, N), dtype=torch.float32, device=rows.device)
-    ws = _bytes(lib.rlpyt_policy_loss_workspace_bytes(code, N, V), rows)
-    with _on(rows) as stream, ktimer.region("action_logp", rows.numel() * rows.element_size()):
-        check(lib.rlpyt_action_logp(code, rows.data_ptr(), rows.stride(0), action.data_ptr(), N, V,
-                                    out[0].data_ptr(), out[1].data_ptr(), ws.data_ptr(), stream),
-              "rlpyt_action_logp")
+    code, device = _DTYPES[rows.dtype], rows.device
     lead = logits.shape[:-1]
-    return out[0].reshape(lead), out[1].reshape(lead)
+    logp = torch.empty(lead, dtype=torch.float32, device=device)
+    entropy = torch.empty(lead, dtype=torch.float32, device=device)
+    ws = _bytes(lib.rlpyt_policy_loss_workspace_bytes(code, N, V), device)
+    _launch(device.index, lib.rlpyt_action_logp, code, rows.data_ptr(), rows.stride(0), action.data_ptr(), N, V,
+            logp.data_ptr(), entropy.data_ptr(), ws.data_ptr())
+    return logp, entropy
 
 
 # --------------------------------------------------------------------------------------
@@ -320,35 +363,46 @@ def orthogonalize(mats, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     ``coeffs`` have to keep singular values of 0 .. 1 bounded (below sqrt(8) on the way).  Not differentiable."""
     single = isinstance(mats, torch.Tensor)
     mats = [mats] if single else list(mats)
-    _need(int(steps) == steps and 1 <= steps <= 100, "orthogonalize: 1 to 100 steps are needed")
-    _need(len(coeffs) == 3, "orthogonalize: three coefficients are needed")
-    _need(eps >= 0., "orthogonalize: eps >= 0 is needed")
+    if int(steps) != steps or not 1 <= steps <= 100:
+        _refuse(f"orthogonalize: 1 to 100 steps are needed, got {steps}")
+    if len(coeffs) != 3:
+        _refuse("orthogonalize: three coefficients are needed")
+    if not eps >= 0.:
+        _refuse("orthogonalize: eps >= 0 is needed")
     for g in mats:
-        _need(g.dim() >= 2 and g.dtype in _DTYPES,
-              f"orthogonalize: matrices in float32, bfloat16 or float16 are needed, got {tuple(g.shape)} {g.dtype}")
+        if g.dim() < 2 or g.dtype not in _DTYPES:
+            _refuse(f"orthogonalize: matrices in float32, bfloat16 or float16 are needed, got {tuple(g.shape)} {g.dtype}")
     if not mats:
         return []
     _need_device("orthogonalize", *mats)
-    outs = [torch.empty(g.shape, dtype=g.dtype, device=g.device) for g in mats]
-    for dtype, code in _DTYPES.items():
-        table, keep = [], []
-        for g, o in zip(mats, outs):
-            if g.dtype != dtype or g.numel() == 0:
-                continue
-            m, n = g.shape[-2:]
-            flat = _unit_rows(g.detach().reshape(-1, m, n))
-            keep.append(flat)
-            size, ld = flat.element_size(), flat.stride(1)
-            table += [(flat.data_ptr() + k * flat.stride(0) * size, ld, o.data_ptr() + k * m * n * size, m, n)
-                      for k in range(flat.shape[0])]
-        if not table:
+    device = mats[0].device
+    outs, tables = [], {}
+    for g in mats:
+        o = torch.empty(g.shape, dtype=g.dtype, device=device)
+        outs.append(o)
+        if g.numel() == 0:
             continue
+        table = tables.setdefault(g.dtype, ([], []))
+        m, n = g.shape[-2:]
+        flat = g.detach()
+        if flat.dim() != 3:
+            flat = flat.reshape(-1, m, n) if flat.dim() > 3 else flat.unsqueeze(0)
+        if flat.stride(-1) != 1 and n != 1:
+            flat = flat.contiguous()
+        table[1].append(flat)
+        size = flat.element_size()
+        src, dst, ld, step = flat.data_ptr(), o.data_ptr(), flat.stride(1), flat.stride(0) * size
+        for k in range(flat.shape[0]):
+            table[0].append((src + k * step, ld, dst + k * m * n * size, m, n))
+    for dtype, (table, _) in tables.items():
         k = len(table)
         ins, lds, dsts, rows, cols = zip(*table)
         ins, dsts = (ctypes.c_void_p * k)(*ins), (ctypes.c_void_p * k)(*dsts)
         lds, rows, cols = ((ctypes.c_int64 * k)(*v) for v in (lds, rows, cols))
-        ws = _bytes(lib.rlpyt_orthogonalize_workspace_bytes(rows, cols, k), keep[0])
-        with _on(keep[0]) as stream, ktimer.region("orthogonalize", 0):
-            check(lib.rlpyt_orthogonalize(code, ins, lds, dsts, rows, cols, k, int(steps), *map(float, coeffs),
-                                          float(eps), ws.data_ptr(), stream), "rlpyt_orthogonalize")
+        ws = _bytes(lib.rlpyt_orthogonalize_workspace_bytes(rows, cols, k), device)
+        _launch(device.index, lib.rlpyt_orthogonalize, _DTYPES[dtype], ins, lds, dsts, rows, cols, k, int(steps),
+                *map(float, coeffs), float(eps), _p(ws))
     return outs[0] if single else outs
+
+
+from .ops import _is_unit_seed  # noqa: E402  (ops imports this module at its end)

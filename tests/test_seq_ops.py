@@ -92,11 +92,10 @@ def test_entry_points_validate_without_a_gpu():
     assert lib.rlpyt_gated_scan_step(0, None, 0, None, 0, None, None, None, 0, 4, None) == 0
     assert lib.rlpyt_gated_scan_step(0, None, 0, None, 0, None, None, None, 2, 4, None) != 0
     loss = lib.rlpyt_policy_kl_loss_fwd_bwd
-    assert loss(0, p, 4, p, p, p, None, None, 2, 0, .2, .2, 0., 0., p, None, None, None, p, None) != 0
-    assert loss(0, None, 4, p, p, p, None, None, 2, 4, .2, .2, 0., 0., p, None, None, None, p, None) != 0
-    assert loss(0, p, 4, p, p, p, None, None, 2, 4, .2, .2, 0., 0., p, p, None, None, p, None) != 0
-    assert b"together" in lib.rlpyt_hip_last_error()
-    assert loss(0, p, 4, p, p, p, None, None, 2, 4, .2, .2, 0., 0., None, None, None, None, p, None) != 0
+    assert loss(0, p, 4, p, p, p, None, None, 2, 0, .2, .2, 0., 0., p, p, None, p, None) != 0
+    assert loss(0, None, 4, p, p, p, None, None, 2, 4, .2, .2, 0., 0., p, p, None, p, None) != 0
+    assert loss(0, p, 4, p, p, p, None, None, 2, 4, .2, .2, 0., 0., None, p, None, p, None) != 0
+    assert loss(0, p, 4, p, p, p, None, None, 2, 4, .2, .2, 0., 0., p, p, None, None, None) != 0
     assert lib.rlpyt_action_logp(0, None, 4, None, 0, 4, None, None, None, None) == 0
     assert lib.rlpyt_action_logp(0, None, 4, None, 2, 4, None, None, None, None) != 0
     assert lib.rlpyt_scale_unless_one(0, None, 0, None, None) == 0
