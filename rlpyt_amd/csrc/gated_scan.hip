@@ -17,7 +17,7 @@
 // (a product of sigmoids is never negative) and composes as "H alone", not as 0 * h.
 //
 // States, maps and sums are 32 bits; x, gate, h and the gradients are f32, bf16 or f16 and each output is
-// rounded once.  The backward pass starts from f32 states kept every kL steps and recomputes the others:
+// rounded once.  The backward pass starts from f32 states kept every kKeep steps and recomputes the others:
 // reading h back would be 2 (4) bytes per element more and, for 16-bit streams, a rounded state.
 #include <algorithm>
 
@@ -26,30 +26,46 @@
 namespace rlpyt {
 namespace {
 
-constexpr int kL = 8;         // steps per wave and window = distance of the kept states
+constexpr int kL = 8;         // steps per wave and window
 constexpr int kMaxWaves = 8;  // waves (consecutive kL-step chunks) per workgroup
+constexpr int kKeep = 32;     // distance of the kept states: every window of 4 or 8 waves starts at one
 
+// V values next to each other, at any multiple of the element's size (global memory asks for no more)
 template <typename E, int V>
 struct Vec {
   typedef E type __attribute__((ext_vector_type(V)));
-  typedef float ftype __attribute__((ext_vector_type(V)));
+  struct __attribute__((packed, aligned(sizeof(E)))) raw { type v; };
 };
+template <typename E, int V>
+__device__ __forceinline__ typename Vec<E, V>::type load(const E* p) {
+  return reinterpret_cast<const typename Vec<E, V>::raw*>(p)->v;
+}
+template <typename E, int V>
+__device__ __forceinline__ void store(E* p, typename Vec<E, V>::type v) {
+  reinterpret_cast<typename Vec<E, V>::raw*>(p)->v = v;
+}
 
 struct Stream {   // one [T, B, D] tensor: unit stride along D, element strides along T and B
   int64_t ts, bs;
 };
 
-// 1 / (1 + e^-g) and its complement, both to f32's relative accuracy
+// z = 1 / (1 + e^-g) and a = 1 - z, both to f32's relative accuracy.  (v_rcp alone leans one way, and the a's go into long
+// products; a large gate is cut where z is 1 and a is nothing beside it; a NaN stays one.)
 __device__ __forceinline__ void gates(float g, float& z, float& a) {
-  const float e = __expf(-fabsf(g));          // NaN gates stay NaN
-  const float r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;
-  z = g >= 0.f ? r : s;
-  a = g >= 0.f ? s : r;
-  if (g != g) z = a = g;
+  float t = g * 1.44269504088896340736f;
+  t = t > 120.f ? 120.f : t;
+  const float e = __builtin_amdgcn_exp2f(t), d = 1.f + e, q = __builtin_amdgcn_rcpf(d);
+  a = fmaf(fmaf(-d, q, 1.f), q, q);
+  z = g > 0.f ? 1.f - a : e * a;
 }
 
 __device__ __forceinline__ float fold(float c, float A, float H) {
-  return A < 0.f ? H : fmaf(A, c, H);
+  return __float_as_int(A) < 0 ? H : fmaf(A, c, H);   // (-0 too: a product behind a reset may vanish)
+}
+
+// A of two maps, one after the other
+__device__ __forceinline__ float chain(float A1, float A2) {
+  return (__float_as_int(A1) | __float_as_int(A2)) < 0 ? -1.f : A1 * A2;
 }
 
 struct Args {
@@ -60,7 +76,7 @@ struct Args {
   float* last;                     // hn (forward) / dh0 (backward) [B D] or null
   const uint8_t* reset;            // [T, B] or null
   const int64_t* lengths;          // [B] or null
-  float* chk;                      // f32 states before steps 0, kL, 2 kL, .. [ceil(T / kL), B D] or null
+  float* chk;                      // f32 states before steps 0, kKeep, 2 kKeep, .. [ceil(T / kKeep), B D] or null
   float2* agg;                     // maps of the segments [S, B D]
   int T, B, D;
   int seg;                         // steps per segment, a multiple of the window
@@ -76,12 +92,14 @@ struct Lane {
 template <int V, bool LEN>
 __device__ __forceinline__ Lane lane_of(const Args& p) {
   Lane l;
-  const int64_t C = (int64_t)p.B * p.D;
-  l.c = ((int64_t)blockIdx.x * kWave + (threadIdx.x & 63)) * V;
-  l.on = l.c < C;                              // V divides D: a lane is in or out as a whole
-  const int64_t c = l.on ? l.c : 0;
-  l.b = (int)(c / p.D);
-  l.d = (int)(c - (int64_t)l.b * p.D);
+  const int per_row = (p.D + V - 1) / V;
+  const int64_t i = (int64_t)blockIdx.x * kWave + (threadIdx.x & 63);
+  l.on = i < (int64_t)p.B * per_row;
+  l.b = l.on ? (int)(i / per_row) : 0;
+  // the last lane of a row of odd length takes a channel of its neighbour again, with the same results
+  l.d = min((int)(i - (int64_t)l.b * per_row) * V, p.D - V);
+  if (!l.on) l.d = 0;
+  l.c = (int64_t)l.b * p.D + l.d;
   l.end = p.T;
   if (LEN) l.end = (int)min((int64_t)p.T, max((int64_t)0, p.lengths[l.b]));
   return l;
@@ -91,21 +109,33 @@ __device__ __forceinline__ Lane lane_of(const Args& p) {
 template <typename E, int V>
 __device__ __forceinline__ void load_chunk(const E* __restrict__ base, int64_t ts, int t0, int last,
                                            typename Vec<E, V>::type (&out)[kL]) {
-  typedef typename Vec<E, V>::type VE;
 #pragma unroll
   for (int i = 0; i < kL; ++i)
-    out[i] = *reinterpret_cast<const VE*>(base + (int64_t)min(t0 + i, last) * ts);
+    out[i] = load<E, V>(base + (int64_t)min(t0 + i, last) * ts);
 }
 
-// Bit i: the state is cleared before step t0 + i.
-__device__ __forceinline__ uint32_t load_resets(const Args& p, const Lane& l, int t0, int end) {
+// The reset bytes of kL steps, fetched like the streams, and as bits: the state is cleared before step t0 + i.
+__device__ __forceinline__ void load_resets(const Args& p, const Lane& l, int t0, uint8_t (&r)[kL]) {
+#pragma unroll
+  for (int i = 0; i < kL; ++i) r[i] = p.reset[(int64_t)min(t0 + i, p.T - 1) * p.B + l.b];
+}
+__device__ __forceinline__ uint32_t reset_bits(const uint8_t (&r)[kL], int t0, int end) {
   uint32_t clear = 0;
 #pragma unroll
-  for (int i = 0; i < kL; ++i) {
-    const bool r = p.reset[(int64_t)min(t0 + i, p.T - 1) * p.B + l.b] != 0;
-    clear |= (uint32_t)(r && t0 + i < end) << i;
-  }
+  for (int i = 0; i < kL; ++i) clear |= (uint32_t)(r[i] != 0 && t0 + i < end) << i;
   return clear;
+}
+
+// Steps behind the end hold the state and add nothing: a gate of -inf (z = 0, a = 1).
+template <typename E, int V>
+__device__ __forceinline__ void mask_chunk(typename Vec<E, V>::type (&gr)[kL], typename Vec<E, V>::type (&other)[kL], int t0,
+                                           int end) {
+#pragma unroll
+  for (int i = 0; i < kL; ++i)
+    if (t0 + i >= end) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) gr[i][k] = (E)-INFINITY, other[i][k] = (E)0.f;
+    }
 }
 
 // The maps before (forward) or behind (backward) segment s, folded into the state this segment starts
@@ -130,7 +160,7 @@ __device__ __forceinline__ void segment_carry(const Args& p, const Lane& l, int 
       for (int k = 0; k < V; ++k) {
         const float2 m = q[k];
         H[k] = fold(H[k], m.x, m.y);
-        A[k] = m.x < 0.f || A[k] < 0.f ? -1.f : A[k] * m.x;
+        A[k] = chain(A[k], m.x);
       }
     }
   }
@@ -171,35 +201,47 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_fwd_kernel(const Ar
   }
   const int step = W * kL;
   VE xr[kL], gr[kL];
+  uint8_t rr[kL];
+  if (RESET) load_resets(p, l, begin + w * kL, rr);
   load_chunk<E, V>(xb, p.xs.ts, begin + w * kL, p.T - 1, xr);
   load_chunk<E, V>(gb, p.gs.ts, begin + w * kL, p.T - 1, gr);
   int buf = 0;
   for (int t0 = begin; t0 < stop; t0 += step, buf ^= 1) {
     const int tc = t0 + w * kL;
     float a[kL][V], b[kL][V], A[V], H[V];
-    const uint32_t clear = RESET ? load_resets(p, l, tc, end) : 0u;
+    const uint32_t clear = RESET ? reset_bits(rr, tc, end) : 0u;
+    // most chunks hold kL steps of every channel and no reset
+    const bool whole = !(LEN ? __any(tc + kL > end) : tc + kL > end), plain = whole && !(RESET && __any(clear != 0));
+    if (!whole) mask_chunk<E, V>(gr, xr, tc, end);
 #pragma unroll
     for (int k = 0; k < V; ++k) A[k] = 1.f, H[k] = 0.f;
 #pragma unroll
-    for (int i = 0; i < kL; ++i) {
-      const bool live = tc + i < end;
+    for (int i = 0; i < kL; ++i)
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        float z, q;
-        gates((float)gr[i][k], z, q);
-        a[i][k] = live ? q : 1.f;
-        b[i][k] = live ? z * (float)xr[i][k] : 0.f;
-        if (RESET && (clear >> i & 1)) {
-          A[k] = -1.f;
-          H[k] = b[i][k];
-        } else {
-          H[k] = fmaf(a[i][k], H[k], b[i][k]);
-          A[k] = A[k] < 0.f ? -1.f : A[k] * a[i][k];
+        float z;
+        gates((float)gr[i][k], z, a[i][k]);
+        b[i][k] = z * (float)xr[i][k];
+      }
+    if (!RESET || plain) {
+#pragma unroll
+      for (int i = 0; i < kL; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) H[k] = fmaf(a[i][k], H[k], b[i][k]), A[k] *= a[i][k];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kL; ++i) {
+        const bool c = clear >> i & 1;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          H[k] = c ? b[i][k] : fmaf(a[i][k], H[k], b[i][k]);
+          A[k] = c ? -1.f : A[k] * a[i][k];     // (keeps its sign)
         }
       }
     }
     // the next window's loads fly over the exchange and the second run
     if (t0 + step < stop) {
+      if (RESET) load_resets(p, l, tc + step, rr);
       load_chunk<E, V>(xb, p.xs.ts, tc + step, p.T - 1, xr);
       load_chunk<E, V>(gb, p.gs.ts, tc + step, p.T - 1, gr);
     }
@@ -214,19 +256,28 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_fwd_kernel(const Ar
       for (int k = 0; k < V; ++k) {
         const float2 m = lds[buf][j][lane * V + k];
         carry[k] = fold(carry[k], m.x, m.y);
-        if (AGG) total[k] = m.x < 0.f || total[k] < 0.f ? -1.f : total[k] * m.x;
+        if (AGG) total[k] = chain(total[k], m.x);
         if (!AGG && j + 1 == w) h[k] = carry[k];
       }
     }
     if (AGG) continue;
-    if (p.chk && tc < stop && l.on) {
-      typedef typename Vec<float, V>::type VF;
-      VF v;
+    if (p.chk && tc % kKeep == 0 && tc < stop && l.on) {
+      typename Vec<float, V>::type v;
 #pragma unroll
       for (int k = 0; k < V; ++k) v[k] = h[k];
-      *reinterpret_cast<VF*>(p.chk + (int64_t)(tc / kL) * C + l.c) = v;
+      store<float, V>(p.chk + (int64_t)(tc / kKeep) * C + l.c, v);
     }
     E* o = hb + (int64_t)tc * p.hs.ts;
+    if (plain) {
+#pragma unroll
+      for (int i = 0; i < kL; ++i) {
+        VE v;
+#pragma unroll
+        for (int k = 0; k < V; ++k) h[k] = fmaf(a[i][k], h[k], b[i][k]), v[k] = (E)h[k];
+        if (l.on) store<E, V>(o + i * p.hs.ts, v);
+      }
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < kL; ++i) {
       VE v;
@@ -236,7 +287,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_fwd_kernel(const Ar
         else h[k] = fmaf(a[i][k], h[k], b[i][k]);
         v[k] = (E)(LEN && tc + i >= end ? 0.f : h[k]);
       }
-      if (tc + i < stop && l.on) *reinterpret_cast<VE*>(o + i * p.hs.ts) = v;
+      if (tc + i < stop && l.on) store<E, V>(o + i * p.hs.ts, v);
     }
   }
   if (w == 0 && l.on) {
@@ -256,6 +307,7 @@ template <typename E, int V, bool RESET, bool LEN, bool AGG>
 __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(const Args p) {
   typedef typename Vec<E, V>::type VE;
   __shared__ float2 lds[2][kMaxWaves][kWave * V];
+  __shared__ float ldh[2][AGG ? 1 : kMaxWaves][kWave * V];   // the maps' H, forward
   const Lane l = lane_of<V, LEN>(p);
   const int lane = threadIdx.x & 63, W = blockDim.x >> 6;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -276,8 +328,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(const Ar
   const int step = W * kL;
   const int windows = (stop - begin + step - 1) / step;
   VE xr[kL], gr[kL], dr[kL];
+  uint8_t rr[kL];
   {
     const int tc = begin + (windows - 1) * step + w * kL;
+    if (RESET) load_resets(p, l, tc, rr);
     if (!AGG) load_chunk<E, V>(xb, p.xs.ts, tc, p.T - 1, xr);
     load_chunk<E, V>(gb, p.gs.ts, tc, p.T - 1, gr);
     load_chunk<E, V>(db, p.hs.ts, tc, p.T - 1, dr);
@@ -285,55 +339,68 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(const Ar
   int buf = 0;
   for (int n = windows - 1; n >= 0; --n, buf ^= 1) {
     const int tc = begin + n * step + w * kL;
-    float a[kL][V], z[kL][V], e[kL][V], d[kL][V], A[V], R[V];
-    const uint32_t clear = RESET ? load_resets(p, l, tc, end) : 0u;
-    float h[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) h[k] = 0.f;
-    if (!AGG && tc < stop && l.on) {
-      typedef typename Vec<float, V>::type VF;
-      const VF v = *reinterpret_cast<const VF*>(p.chk + (int64_t)(tc / kL) * C + l.c);
+    float a[kL][V], z[kL][V], x[kL][V], d[kL][V], A[V], R[V], H[V];
+    const uint32_t clear = RESET ? reset_bits(rr, tc, end) : 0u;
+    const bool whole = !(LEN ? __any(tc + kL > end) : tc + kL > end), plain = whole && !(RESET && __any(clear != 0));
+    if (!whole) {
+      mask_chunk<E, V>(gr, dr, tc, end);
+      if (!AGG) mask_chunk<E, V>(gr, xr, tc, end);
+    }
+    float h[V];                    // the state this window starts from; every wave folds up to its own steps
+    if (!AGG) {
+      const typename Vec<float, V>::type v = load<float, V>(p.chk + (int64_t)((tc - w * kL) / kKeep) * C + l.c);
 #pragma unroll
       for (int k = 0; k < V; ++k) h[k] = v[k];
     }
 #pragma unroll
-    for (int i = 0; i < kL; ++i) {
-      const bool live = tc + i < end;
+    for (int k = 0; k < V; ++k) A[k] = 1.f, R[k] = 0.f, H[k] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kL; ++i)
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         gates((float)gr[i][k], z[i][k], a[i][k]);
-        if (!live) a[i][k] = 1.f, z[i][k] = 0.f;
-        d[i][k] = live ? (float)dr[i][k] : 0.f;
-        if (!AGG) {
-          if (RESET && (clear >> i & 1)) h[k] = 0.f;
-          const float x = live ? (float)xr[i][k] : 0.f;
-          e[i][k] = (x - h[k]) * z[i][k] * a[i][k];
-          h[k] = fmaf(a[i][k], h[k], z[i][k] * x);
+        d[i][k] = (float)dr[i][k];
+        if (!AGG) x[i][k] = (float)xr[i][k];
+      }
+    if (!RESET || plain) {
+#pragma unroll
+      for (int i = kL - 1; i >= 0; --i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) R[k] = a[i][k] * (d[i][k] + R[k]), A[k] *= a[i][k];
+      if (!AGG)
+#pragma unroll
+        for (int i = 0; i < kL; ++i)
+#pragma unroll
+          for (int k = 0; k < V; ++k) H[k] = fmaf(a[i][k], H[k], z[i][k] * x[i][k]);
+    } else {
+#pragma unroll
+      for (int i = kL - 1; i >= 0; --i) {
+        const bool c = clear >> i & 1;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          R[k] = c ? 0.f : a[i][k] * (d[i][k] + R[k]);
+          A[k] = c ? -1.f : A[k] * a[i][k];     // (keeps its sign)
         }
       }
-    }
+      if (!AGG)
 #pragma unroll
-    for (int k = 0; k < V; ++k) A[k] = 1.f, R[k] = 0.f;
+        for (int i = 0; i < kL; ++i) {
+          const bool c = clear >> i & 1;
 #pragma unroll
-    for (int i = kL - 1; i >= 0; --i) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        if (RESET && (clear >> i & 1)) {
-          A[k] = -1.f;
-          R[k] = 0.f;
-        } else {
-          R[k] = a[i][k] * (d[i][k] + R[k]);
-          A[k] = A[k] < 0.f ? -1.f : A[k] * a[i][k];
+          for (int k = 0; k < V; ++k) H[k] = fmaf(a[i][k], c ? 0.f : H[k], z[i][k] * x[i][k]);
         }
-      }
     }
     if (n > 0) {
+      if (RESET) load_resets(p, l, tc - step, rr);
       if (!AGG) load_chunk<E, V>(xb, p.xs.ts, tc - step, p.T - 1, xr);
       load_chunk<E, V>(gb, p.gs.ts, tc - step, p.T - 1, gr);
       load_chunk<E, V>(db, p.hs.ts, tc - step, p.T - 1, dr);
     }
 #pragma unroll
-    for (int k = 0; k < V; ++k) lds[buf][w][lane * V + k] = float2{A[k], R[k]};
+    for (int k = 0; k < V; ++k) {
+      lds[buf][w][lane * V + k] = float2{A[k], R[k]};
+      if (!AGG) ldh[buf][w][lane * V + k] = H[k];
+    }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < V; ++k) R[k] = carry[k];
@@ -342,13 +409,52 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(const Ar
       for (int k = 0; k < V; ++k) {
         const float2 m = lds[buf][j][lane * V + k];
         carry[k] = fold(carry[k], m.x, m.y);
-        if (AGG) total[k] = m.x < 0.f || total[k] < 0.f ? -1.f : total[k] * m.x;
+        if (AGG) total[k] = chain(total[k], m.x);
         if (!AGG && j - 1 == w) R[k] = carry[k];
       }
     }
     if (AGG) continue;
+    for (int j = 0; j < w; ++j)
+#pragma unroll
+      for (int k = 0; k < V; ++k) h[k] = fold(h[k], lds[buf][j][lane * V + k].x, ldh[buf][j][lane * V + k]);
     E* ox = (E*)p.dx + (int64_t)l.b * p.dxs.bs + l.d + (int64_t)tc * p.dxs.ts;
     E* og = (E*)p.dgate + (int64_t)l.b * p.dgs.bs + l.d + (int64_t)tc * p.dgs.ts;
+    // x becomes dgate_t / G_t
+    if (plain) {
+#pragma unroll
+      for (int i = 0; i < kL; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float b = z[i][k] * x[i][k];
+          x[i][k] = (x[i][k] - h[k]) * (z[i][k] * a[i][k]);
+          h[k] = fmaf(a[i][k], h[k], b);
+        }
+#pragma unroll
+      for (int i = kL - 1; i >= 0; --i) {
+        VE vx, vg;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float G = d[i][k] + R[k];
+          vx[k] = (E)(z[i][k] * G);
+          vg[k] = (E)(x[i][k] * G);
+          R[k] = a[i][k] * G;
+        }
+        if (l.on) {
+          store<E, V>(ox + i * p.dxs.ts, vx);
+          store<E, V>(og + i * p.dgs.ts, vg);
+        }
+      }
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < kL; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        if (RESET && (clear >> i & 1)) h[k] = 0.f;
+        const float b = z[i][k] * x[i][k];
+        x[i][k] = (x[i][k] - h[k]) * (z[i][k] * a[i][k]);
+        h[k] = fmaf(a[i][k], h[k], b);
+      }
 #pragma unroll
     for (int i = kL - 1; i >= 0; --i) {
       VE vx, vg;
@@ -357,12 +463,12 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(const Ar
         const bool live = !LEN || tc + i < end;
         const float G = d[i][k] + R[k];
         vx[k] = (E)(live ? z[i][k] * G : 0.f);
-        vg[k] = (E)(live ? e[i][k] * G : 0.f);
+        vg[k] = (E)(live ? x[i][k] * G : 0.f);
         R[k] = RESET && (clear >> i & 1) ? 0.f : a[i][k] * G;
       }
       if (tc + i < stop && l.on) {
-        *reinterpret_cast<VE*>(ox + i * p.dxs.ts) = vx;
-        *reinterpret_cast<VE*>(og + i * p.dgs.ts) = vg;
+        store<E, V>(ox + i * p.dxs.ts, vx);
+        store<E, V>(og + i * p.dgs.ts, vg);
       }
     }
   }
@@ -411,22 +517,27 @@ struct Plan {
   int W, S, seg;
 };
 
-// W: waves that share the channels of one tile, at most kMaxWaves.  S: segments along time.  A single
-// segment reads the streams once; S > 1 reads them twice and adds a launch, so it is taken only where the tiles alone
-// leave most of the 256 CUs idle.
+// A lane takes 4 bytes of a row: two 16-bit channels.  (8 bytes of f32: 192 registers, and a scan of 85 x 32 x 512 took 24 us
+// both ways instead of 20.)
+int channels(int size, int64_t D) { return size == 2 && D > 1 ? 2 : 1; }
+int64_t tiles_of(int64_t B, int64_t D, int V) { return ceil_div(B * ceil_div(D, V), kWave); }
+
+// W: waves that share the channels of one tile: 4 where the tiles fill the chip, else 8 (or what T needs).  S: segments
+// along time.  A single segment reads the streams once; S > 1 reads them twice and adds a launch, so it is taken only where
+// the tiles alone leave many of the 256 CUs idle (128 tiles of 2048 steps: 190 us in one segment, 175 in four).
 Plan plan_of(int64_t T, int64_t tiles) {
   Plan q;
-  q.W = (int)std::min<int64_t>(kMaxWaves, std::max<int64_t>(1, ceil_div(T, kL)));
+  q.W = (int)std::min<int64_t>(tiles >= 512 ? 4 : kMaxWaves, std::max<int64_t>(1, ceil_div(T, kL)));
   const int64_t window = (int64_t)q.W * kL, windows = std::max<int64_t>(1, ceil_div(T, window));
   int64_t S = 1;
-  if (tiles < 128) S = std::min<int64_t>({windows, ceil_div(512, tiles), (int64_t)256});
+  if (tiles < 192) S = std::min<int64_t>({windows, ceil_div(512, tiles), (int64_t)256});
   const int64_t seg = ceil_div(windows, S) * window;
   q.S = (int)std::max<int64_t>(1, ceil_div(T, seg));
   q.seg = (int)std::min<int64_t>(seg, (int64_t)1 << 30);
   return q;
 }
 
-// The widest vector (<= 4 bytes of 16-bit, 4 .. 8 bytes of f32 elements) that every row start is aligned to.
+// Whether every row start is aligned to V elements.
 bool fits(const void* ptr, Stream st, int D, int V, int size) {
   return ((uintptr_t)ptr & (V * size - 1)) == 0 && st.ts % V == 0 && st.bs % V == 0 && D % V == 0;
 }
@@ -447,7 +558,7 @@ int launch(const Args& p, const Plan& q, int64_t tiles, hipStream_t s) {
 
 template <bool FWD, typename E, int V>
 int dispatch(const Args& p, hipStream_t s) {
-  const int64_t tiles = ceil_div((int64_t)p.B * p.D, (int64_t)kWave * V);
+  const int64_t tiles = tiles_of(p.B, p.D, V);
   const Plan q = plan_of(p.T, tiles);
   Args a = p;
   a.seg = q.seg;
@@ -459,11 +570,9 @@ int dispatch(const Args& p, hipStream_t s) {
 
 template <bool FWD, typename E>
 int pick(const Args& p, hipStream_t s) {
-  const int size = (int)sizeof(E);
-  const bool wide = fits(p.x, p.xs, p.D, 2, size) && fits(p.gate, p.gs, p.D, 2, size) &&
-                    fits(FWD ? p.h : p.dh, p.hs, p.D, 2, size) &&
-                    (FWD || (fits(p.dx, p.dxs, p.D, 2, size) && fits(p.dgate, p.dgs, p.D, 2, size)));
-  if (wide) return dispatch<FWD, E, 2>(p, s);
+  if constexpr (sizeof(E) == 2) {
+    if (channels(2, p.D) == 2) return dispatch<FWD, E, 2>(p, s);
+  }
   return dispatch<FWD, E, 1>(p, s);
 }
 
@@ -478,14 +587,12 @@ bool sizes_ok(int64_t T, int64_t B, int64_t D) {
 
 using namespace rlpyt;
 
-extern "C" int64_t rlpyt_gated_scan_state_rows(int64_t T) { return T <= 0 ? 0 : ceil_div(T, kL); }
+extern "C" int64_t rlpyt_gated_scan_state_rows(int64_t T) { return T <= 0 ? 0 : ceil_div(T, kKeep); }
 
 extern "C" int64_t rlpyt_gated_scan_workspace_bytes(int64_t T, int64_t B, int64_t D) {
   if (!sizes_ok(T, B, D) || T == 0 || B == 0 || D == 0) return 0;
-  // the narrow variant has more tiles, hence fewer segments: the wide one's count bounds both
-  const Plan q = plan_of(T, ceil_div(B * D, (int64_t)kWave * 2));
-  const Plan n = plan_of(T, ceil_div(B * D, (int64_t)kWave));
-  const int64_t S = std::max(q.S, n.S);
+  int64_t S = 1;      // (of either element size)
+  for (int size : {2, 4}) S = std::max<int64_t>(S, plan_of(T, tiles_of(B, D, channels(size, D))).S);
   return S > 1 ? S * B * D * (int64_t)sizeof(float2) : 0;
 }
 

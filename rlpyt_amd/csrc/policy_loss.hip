@@ -6,15 +6,15 @@
 //   loss = sum_n w_n (pi + c_kl kl - c_H H) / sum_n w_n
 //   dl_j = w / sum w [ c 1_{j = a} + p_j (c_H (log p_j + H) - c) ]     c = dpi/dlogp - c_kl (e^d - 1)
 //
-// Memory bound: the floor reads and writes the logits once.  A row is kept in registers (a group of lanes for
-// V <= 1024, a workgroup up to 256 KB a row) between the softmax statistics and the gradient.  Longer rows,
+// Memory bound: the floor reads and writes the logits once.  A row is kept in registers (of a group of lanes for
+// V <= 128, of a wave up to 4 KB, of a workgroup up to 256 KB) between the softmax statistics and the gradient.  Longer rows,
 // and batches of so few rows that one workgroup each leaves the chip idle, are split over workgroups: one
 // launch for the statistics of the parts, one that joins them and reads the row again for the gradient.
 //
-// Sums over a row are f32 per lane and in a fixed order (no atomics); log(sum) and everything per row is 64 bits:
-// kl ~ d^2 / 2 cancels in 32.  x - max is formed before it is scaled for exp2, so that the error of e^(x - max) goes with
-// its exponent and not with the logit.  A difference below -200 counts as -200 (its e^ is 0 in f32), which keeps
-// 0 * log 0 = 0 for logits of -inf; NaN goes through to the loss.
+// Sums over a row are f32 per lane and in a fixed order (no atomics); what is done once per row is in 64 bits, on f32
+// logarithms and exponentials of reduced arguments: kl ~ d^2 / 2 cancels in 32.  Exponents are in base 2 and come from one fma,
+// t = x log2(e) - m with m the rounded product of the largest logit; what that rounding took is put back per row.  -inf
+// logits: t = -inf, e^t = 0, and 0 * t is kept 0 by taking t no lower than -300.  NaN goes through to the loss.
 #include <math.h>
 
 #include <algorithm>
@@ -47,23 +47,22 @@ struct LossArgs {
 };
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kFloor = -200.f;   // e^-200 is 0 in f32
+constexpr double kLn2 = 0.69314718055994530942;
+constexpr float kFloor = -300.f;   // 2^-300 is 0 in f32
 
-__device__ __forceinline__ float below(float x, float m) {
-  const float t = x - m;
-  return t < kFloor ? kFloor : t;  // (NaN stays NaN)
-}
-__device__ __forceinline__ float exp_of(float t) { return __builtin_amdgcn_exp2f(t * kLog2e); }
+__device__ __forceinline__ float exp_of(float t) { return __builtin_amdgcn_exp2f(t); }
+__device__ __forceinline__ float bounded(float t) { return fmaxf(t, kFloor); }
 
-// Softmax statistics of some logits: s = sum e^(x - m), u = sum e^(x - m) (x - m); m = -inf: none.
+// Softmax statistics of some logits: with t = x log2(e) - m,  s = sum 2^t,  u = sum 2^t t; m = -inf: none.
 struct Stats {
   float m, s, u;
 };
+__device__ __forceinline__ float scaled(float largest) { return largest * kLog2e; }
 __device__ __forceinline__ Stats join(const Stats& p, const Stats& q) {
   Stats r;
   r.m = fmaxf(p.m, q.m);
   if (r.m == -INFINITY) return Stats{-INFINITY, p.s + q.s, 0.f};   // (NaN sums stay)
-  const float dp = below(p.m, r.m), dq = below(q.m, r.m), fp = exp_of(dp), fq = exp_of(dq);
+  const float dp = bounded(p.m - r.m), dq = bounded(q.m - r.m), fp = exp_of(dp), fq = exp_of(dq);
   r.s = fmaf(fp, p.s, fq * q.s);
   r.u = fp * fmaf(dp, p.s, p.u) + fq * fmaf(dq, q.s, q.u);
   return r;
@@ -85,27 +84,43 @@ __device__ __forceinline__ float group_max(float m) {
   return m;
 }
 
-// What follows from a row's statistics: its terms of the loss, and its gradient as e^t (k1 t + k0), + ka at the action.
+// log(s) to 2^-24 absolute: s = 2^k f with f in [1, 2)
+__device__ __forceinline__ double log_of(float s) {
+  const int k = (int)(__float_as_uint(s) >> 23) - 127;
+  if (!(s >= 1.f && s < 3e38f)) return log((double)s);   // (the largest term of a row's sum is 1)
+  return (double)k * kLn2 + (double)logf(__uint_as_float((__float_as_uint(s) & 0x7fffffu) | 0x3f800000u));
+}
+// e^d - d - 1 >= 0, to ~ 2^-20 relative: the series where it cancels
+__device__ __forceinline__ double kl_of(double d) {
+  if (fabs(d) > 0.5) return (double)expf((float)d) - d - 1.0;
+  double v = 1.0;                     // d^12 / 12! is left out
+#pragma unroll
+  for (int k = 11; k >= 3; --k) v = fma(v, d * (1.0 / k), 1.0);
+  return 0.5 * d * d * v;
+}
+
+// What follows from a row's statistics: its terms of the loss, and its gradient as 2^t (k1 t + k0), + ka at the action.
 struct RowOut {
   double pi, kl, ent, clipped;
   float logp, entropy, m, k1, k0, ka;
 };
-__device__ __forceinline__ RowOut row_terms(const LossArgs& p, int64_t n, float w, const Stats& st,
-                                            bool some, float xa, bool in_range) {
+__device__ __forceinline__ RowOut row_terms(const LossArgs& p, int64_t n, float w, const Stats& st, float xa,
+                                            bool in_range) {
   RowOut o = {};
   o.m = st.m;
-  if (!some) {   // every logit is -inf: no distribution, the row adds nothing and has no gradient
+  if (st.m == -INFINITY && st.s == 0.f) {   // every logit is -inf: no distribution, the row adds nothing and has no gradient
     o.m = 0.f;
     o.logp = -INFINITY;
     return o;
   }
-  const double logs = log((double)st.s);
-  const double H = logs - (double)st.u / (double)st.s;
-  const double lp = in_range ? ((double)xa - (double)st.m) - logs : (double)NAN;
+  // natural logarithms: x - lse = (x log2(e) - m) ln 2 - log(s)
+  const double logs = log_of(st.s), mean = (double)st.u / (double)st.s * kLn2;
+  const double H = logs - mean;
+  const double lp = in_range ? ((double)xa * (double)kLog2e - (double)st.m) * kLn2 - logs : (double)NAN;
   o.logp = (float)lp;
   o.entropy = (float)H;
   if (!p.rows) return o;
-  const double A = (double)p.advantage[n], r = exp(lp - (double)p.old_logp[n]);
+  const double A = (double)p.advantage[n], r = (double)expf((float)(lp - (double)p.old_logp[n]));
   const double rc = fmin(fmax(r, 1.0 - p.lo), 1.0 + p.hi);
   double c = 0.0;
   if (A != 0.0 || r != r) {
@@ -116,21 +131,21 @@ __device__ __forceinline__ RowOut row_terms(const LossArgs& p, int64_t n, float 
   }
   o.clipped = r != rc ? 1.0 : 0.0;
   if (p.ref_logp) {
-    const double d = (double)p.ref_logp[n] - lp, e = expm1(d);
-    o.kl = e - d;
-    c -= p.c_kl * e;
+    const double d = (double)p.ref_logp[n] - lp;
+    o.kl = kl_of(d);
+    c -= p.c_kl * (o.kl + d);
   }
   o.ent = H;
   const double denom = p.denom ? *p.denom : (double)p.N;
   const double g = denom > 0.0 ? (double)w / denom : 0.0, gs = g / (double)st.s;
-  o.k1 = (float)(gs * p.c_ent);
+  o.k1 = (float)(gs * p.c_ent * kLn2);
   o.k0 = (float)(gs * (p.c_ent * (H - logs) - c));
   o.ka = (float)(g * c);
   o.pi *= w, o.kl *= w, o.ent *= w, o.clipped *= w;
   return o;
 }
 
-// ---- V <= 16 G: G lanes a row, K elements a lane ---------------------------------------------------------
+// ---- V <= 4 G: G lanes a row, K elements a lane ---------------------------------------------------------
 template <typename E, int G, int K>
 __global__ __launch_bounds__(256) void loss_group_kernel(const LossArgs p) {
   __shared__ double sums[4 * 16];
@@ -149,13 +164,13 @@ __global__ __launch_bounds__(256) void loss_group_kernel(const LossArgs p) {
       x[k] = live && j < p.V ? (float)row[j] : -INFINITY;
       m = fmaxf(m, x[k]);
     }
-    m = group_max<G>(m);
-    Stats st = {m, 0.f, 0.f};
+    Stats st = {scaled(group_max<G>(m)), 0.f, 0.f};
+    const float from = st.m == -INFINITY ? 0.f : st.m;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const float t = below(x[k], m == -INFINITY ? 0.f : m), e = exp_of(t);
+      const float t = fmaf(x[k], kLog2e, -from), e = exp_of(t);
       st.s += e;
-      st.u = fmaf(e, t, st.u);
+      st.u = fmaf(e, bounded(t), st.u);
     }
 #pragma unroll
     for (int o2 = G / 2; o2 > 0; o2 >>= 1) {
@@ -165,7 +180,7 @@ __global__ __launch_bounds__(256) void loss_group_kernel(const LossArgs p) {
     if (live) {
       const int64_t a = p.action[n];
       const bool in_range = a >= 0 && a < p.V;
-      o = row_terms(p, n, w, st, !(m == -INFINITY && st.s == 0.f), in_range ? (float)row[a] : 0.f, in_range);
+      o = row_terms(p, n, w, st, in_range ? (float)row[a] : 0.f, in_range);
       if (p.logp && sub == 0) p.logp[n] = o.logp, p.entropy[n] = o.entropy;
     }
     if (p.grad) {
@@ -174,8 +189,8 @@ __global__ __launch_bounds__(256) void loss_group_kernel(const LossArgs p) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int j = sub + k * G;
-        const float t = below(x[k], o.m), e = exp_of(t);
-        float v = e * fmaf(o.k1, t, o.k0);
+        const float t = fmaf(x[k], kLog2e, -o.m);
+        float v = exp_of(t) * fmaf(o.k1, bounded(t), o.k0);
         if (j == a) v += o.ka;
         if (j < p.V) g[j] = (E)(live ? v : 0.f);
       }
@@ -215,35 +230,52 @@ template <typename E>
 __device__ __forceinline__ typename Row16<E>::vec grad16(typename Row16<E>::vec x, int j, int64_t a,
                                                          const RowOut& o) {
   constexpr int n = Row16<E>::n;
-  typename Row16<E>::vec v;
+  float g[n];
 #pragma unroll
   for (int k = 0; k < n; ++k) {
-    const float t = below((float)x[k], o.m), e = exp_of(t);
-    float g = e * fmaf(o.k1, t, o.k0);
-    if (j + k == a) g += o.ka;
-    v[k] = (E)g;
+    const float t = fmaf((float)x[k], kLog2e, -o.m);
+    g[k] = exp_of(t) * fmaf(o.k1, bounded(t), o.k0);
   }
+  if ((uint64_t)(a - j) < (uint64_t)n) {
+#pragma unroll
+    for (int k = 0; k < n; ++k)
+      if (j + k == a) g[k] += o.ka;
+  }
+  typename Row16<E>::vec v;
+#pragma unroll
+  for (int k = 0; k < n; ++k) v[k] = (E)g[k];
   return v;
+}
+// Keeps the compiler from holding the floats of one pass over a row's registers for the next: they are converted again, and
+// two workgroups of 1024 fit a CU, one loading while the other computes.
+template <typename E, int R>
+__device__ __forceinline__ void forget(typename Row16<E>::vec (&x)[R]) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    uint4 v = __builtin_bit_cast(uint4, x[r]);
+    asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));
+    x[r] = __builtin_bit_cast(typename Row16<E>::vec, v);
+  }
 }
 // statistics of the vectors of a wave
 template <typename E, int R>
-__device__ __forceinline__ Stats wave_stats(const typename Row16<E>::vec (&x)[R]) {
+__device__ __forceinline__ Stats wave_stats(typename Row16<E>::vec (&x)[R]) {
   constexpr int n = Row16<E>::n;
   float m = -INFINITY;
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int k = 0; k < n; ++k) m = fmaxf(m, (float)x[r][k]);
-  m = group_max<kWave>(m);
-  Stats st = {m, 0.f, 0.f};
-  const float from = m == -INFINITY ? 0.f : m;
+  forget<E, R>(x);
+  Stats st = {scaled(group_max<kWave>(m)), 0.f, 0.f};
+  const float from = st.m == -INFINITY ? 0.f : st.m;
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int k = 0; k < n; ++k) {
-      const float t = below((float)x[r][k], from), e = exp_of(t);
+      const float t = fmaf((float)x[r][k], kLog2e, -from), e = exp_of(t);
       st.s += e;
-      st.u = fmaf(e, t, st.u);
+      st.u = fmaf(e, bounded(t), st.u);
     }
   st.s = wave_sum(st.s);
   st.u = wave_sum(st.u);
@@ -292,8 +324,9 @@ __global__ __launch_bounds__(NT) void loss_row_kernel(const LossArgs p) {
 #pragma unroll
   for (int r = 0; r < R; ++r) x[r] = load16<E>(row, (r * NT + threadIdx.x) * n16, p.V);
   const Stats st = block_join<NT>(wave_stats<E, R>(x), lds);
+  forget<E, R>(x);
   if (threadIdx.x == 0) {
-    out = row_terms(p, n, w, st, !(st.m == -INFINITY && st.s == 0.f), xa, in_range);
+    out = row_terms(p, n, w, st, xa, in_range);
     if (p.logp) p.logp[n] = out.logp, p.entropy[n] = out.entropy;
     if (p.rows) p.rows[n * 4] = out.pi, p.rows[n * 4 + 1] = out.kl, p.rows[n * 4 + 2] = out.ent, p.rows[n * 4 + 3] = out.clipped;
   }
@@ -304,6 +337,51 @@ __global__ __launch_bounds__(NT) void loss_row_kernel(const LossArgs p) {
   for (int r = 0; r < R; ++r) {
     const int j = (r * NT + threadIdx.x) * n16;
     if (j < p.V) store16<E>(g, j, p.V, grad16<E>(x[r], j, a, o));
+  }
+}
+
+// ---- a row held by one wave, R x 16 bytes a lane ----------------------------------------------------------
+template <typename E, int R>
+__global__ __launch_bounds__(256) void loss_wave_kernel(const LossArgs p) {
+  typedef typename Row16<E>::vec vec;
+  constexpr int n16 = Row16<E>::n;
+  __shared__ double sums[4][4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t n = p.n0 + (int64_t)blockIdx.x * 4 + wave;
+  const bool on = n < p.n0 + p.n_rows;
+  const float w = on ? (p.valid ? p.valid[n] : 1.f) : 0.f;
+  RowOut o = {};
+  if (w != 0.f) {
+    const E* row = (const E*)p.logits + n * p.row_stride;
+    const int64_t a = p.action[n];
+    const bool in_range = a >= 0 && a < p.V;
+    const float xa = in_range ? (float)row[a] : 0.f;
+    vec x[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[r] = load16<E>(row, (r * kWave + lane) * n16, p.V);
+    o = row_terms(p, n, w, wave_stats<E, R>(x), xa, in_range);
+    forget<E, R>(x);
+    if (lane == 0 && p.logp) p.logp[n] = o.logp, p.entropy[n] = o.entropy;
+    if (p.grad) {
+      E* g = (E*)p.grad + n * p.V;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int j = (r * kWave + lane) * n16;
+        if (j < p.V) store16<E>(g, j, p.V, grad16<E>(x[r], j, a, o));
+      }
+    }
+  } else if (on && p.grad) {
+    vec zero;
+#pragma unroll
+    for (int k = 0; k < n16; ++k) zero[k] = (E)0.f;
+    for (int j = lane * n16; j < p.V; j += kWave * n16) store16<E>((E*)p.grad + n * p.V, j, p.V, zero);
+  }
+  if (!p.rows) return;
+  if (lane == 0) sums[0][wave] = o.pi, sums[1][wave] = o.kl, sums[2][wave] = o.ent, sums[3][wave] = o.clipped;
+  __syncthreads();
+  if (threadIdx.x < 4) {
+    const double* v = sums[threadIdx.x];
+    p.rows[(p.n0 / 4 + blockIdx.x) * 4 + threadIdx.x] = v[0] + v[1] + v[2] + v[3];
   }
 }
 
@@ -353,7 +431,7 @@ __global__ __launch_bounds__(kSplitThreads) void loss_join_kernel(const LossArgs
     st = block_join<kSplitThreads>(group_join<kWave>(st), lds);
     if (threadIdx.x == 0) {
       const bool in_range = a >= 0 && a < p.V;
-      out = row_terms(p, n, w, st, !(st.m == -INFINITY && st.s == 0.f), in_range ? (float)row[a] : 0.f, in_range);
+      out = row_terms(p, n, w, st, in_range ? (float)row[a] : 0.f, in_range);
       if (first && p.logp) p.logp[n] = out.logp, p.entropy[n] = out.entropy;
     }
   } else if (threadIdx.x == 0) {
@@ -428,26 +506,31 @@ __global__ __launch_bounds__(256) void loss_scale_kernel(E* __restrict__ g, int6
 
 // ------------------------------------------------------------------------------------ host side
 enum { F32 = 0, BF16 = 1, F16 = 2 };
-constexpr int kGroupV = 1024;       // longest row of the lane groups
+constexpr int kGroupV = 128;        // longest row of the lane groups
+constexpr int kWaveBytes = 4096;    // and of a wave
 
 struct LossPlan {
   int P, part;                      // P > 0: rows split into P parts of `part` elements
   int64_t partials;                 // rows of the [., 4] table of partial sums
 };
-int group_lanes(int64_t V) { return V <= 32 ? 8 : V <= 64 ? 16 : V <= 128 ? 32 : 64; }
+int group_lanes(int64_t V) { return V <= 32 ? 8 : V <= 64 ? 16 : 32; }
 
-// A row goes to one workgroup while it fits its registers (256 KB) and the rows fill the chip; otherwise it is split into parts of
-// at least 8 KB so that there are about 1024 workgroups.  The split reads the row twice: it pays below ~128 rows.
+// A row goes to a group of lanes, a wave or a workgroup (256 KB at most) whose registers hold it, while the rows fill the chip;
+// otherwise it is split into parts of at least 8 KB so that there are about 1024 workgroups.
 LossPlan plan_of(int64_t N, int64_t V, int size) {
   LossPlan q = {0, 0, N};
   if (V <= kGroupV) {
     q.partials = ceil_div(N, 256 / group_lanes(V));
     return q;
   }
+  if (V * size <= kWaveBytes) {
+    q.partials = ceil_div(N, 4);
+    return q;
+  }
   const bool held = V * size <= 256 * 1024;
-  if (held && (N >= 128 || V * size <= 16 * 1024)) return q;
-  const int64_t least = ceil_div(V * size, 8 * 1024), want = std::max<int64_t>(1, ceil_div(1024, N));
-  const int64_t P = std::max<int64_t>(1, std::min(least, std::max<int64_t>(want, held ? 1 : 4)));
+  if (held && (N >= 256 || V * size <= 16 * 1024)) return q;
+  const int64_t least = ceil_div(V * size, 8 * 1024), want = std::max<int64_t>(held ? 1 : 4, ceil_div(1024, N));
+  const int64_t P = std::min(least, want);
   q.part = (int)(ceil_div(ceil_div(V, P), 8) * 8);
   q.P = (int)ceil_div(V, q.part);
   return q;
@@ -456,17 +539,20 @@ LossPlan plan_of(int64_t N, int64_t V, int size) {
 template <typename E>
 int run(LossArgs p, const LossPlan& q, hipStream_t s) {
   const int V = p.V;
+  const int64_t vecs = ceil_div((int64_t)V, (int64_t)Row16<E>::n);
   if (V <= kGroupV) {
     const dim3 grid((unsigned)ceil_div(p.n_rows, 256 / group_lanes(V)));
     if (V <= 8) RL_LAUNCH((loss_group_kernel<E, 8, 1>), grid, dim3(256), 0, s, p);
     else if (V <= 32) RL_LAUNCH((loss_group_kernel<E, 8, 4>), grid, dim3(256), 0, s, p);
     else if (V <= 64) RL_LAUNCH((loss_group_kernel<E, 16, 4>), grid, dim3(256), 0, s, p);
-    else if (V <= 128) RL_LAUNCH((loss_group_kernel<E, 32, 4>), grid, dim3(256), 0, s, p);
-    else if (V <= 256) RL_LAUNCH((loss_group_kernel<E, 64, 4>), grid, dim3(256), 0, s, p);
-    else RL_LAUNCH((loss_group_kernel<E, 64, 16>), grid, dim3(256), 0, s, p);
+    else RL_LAUNCH((loss_group_kernel<E, 32, 4>), grid, dim3(256), 0, s, p);
+  } else if (V * (int64_t)sizeof(E) <= kWaveBytes) {
+    const dim3 grid((unsigned)ceil_div(p.n_rows, 4));
+    if (vecs <= 64) RL_LAUNCH((loss_wave_kernel<E, 1>), grid, dim3(256), 0, s, p);
+    else if (vecs <= 128) RL_LAUNCH((loss_wave_kernel<E, 2>), grid, dim3(256), 0, s, p);
+    else RL_LAUNCH((loss_wave_kernel<E, 4>), grid, dim3(256), 0, s, p);
   } else if (q.P == 0) {
     const dim3 grid((unsigned)p.n_rows);
-    const int64_t vecs = ceil_div((int64_t)V, (int64_t)Row16<E>::n);
     if (vecs <= 512) RL_LAUNCH((loss_row_kernel<E, 256, 2>), grid, dim3(256), 0, s, p);
     else if (vecs <= 1024) RL_LAUNCH((loss_row_kernel<E, 256, 4>), grid, dim3(256), 0, s, p);
     else if (vecs <= 2048) RL_LAUNCH((loss_row_kernel<E, 512, 4>), grid, dim3(512), 0, s, p);
@@ -570,7 +656,7 @@ extern "C" int rlpyt_scale_unless_one(int dtype, void* x, int64_t n, const float
   RL_CHECK_ARG(RL_ALIGNED16(x), RLPYT_ESHAPE, "rlpyt_scale_unless_one: x must be 16-byte aligned");
   hipStream_t s = (hipStream_t)stream;
   const int per = 256 * (16 / element_size(dtype));
-  const dim3 grid((unsigned)std::min<int64_t>(2048, ceil_div(n, per)));
+  const dim3 grid((unsigned)std::min<int64_t>(1024, ceil_div(n, per)));
   if (dtype == F32) RL_LAUNCH((loss_scale_kernel<float>), grid, dim3(256), 0, s, (float*)x, n, scale);
   else if (dtype == BF16) RL_LAUNCH((loss_scale_kernel<__bf16>), grid, dim3(256), 0, s, (__bf16*)x, n, scale);
   else RL_LAUNCH((loss_scale_kernel<_Float16>), grid, dim3(256), 0, s, (_Float16*)x, n, scale);
