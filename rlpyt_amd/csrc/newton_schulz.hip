@@ -47,19 +47,15 @@ struct Mat {
 };
 // The first launch gets the table as its argument and leaves it in the workspace for the others: an argument is read from the
 // host's memory, 3 KB of it by every launch.
-enum { LOAD = 0, SYM = 1, FULL = 2 };
+enum { LOAD = 0, SYM = 1, FULL = 4, KINDS = 7 };   // (SYM, FULL: + 0, 1, 2 for tiles of 64, 128, 256)
 struct Mats {
   Mat m[kMats];
-  int first[3][kMats];               // first tile of a matrix: of ns_load_kernel, of symmetric and of full products; INT_MAX behind n
+  int first[KINDS][kMats];           // first tile of a matrix: of ns_load_kernel, of symmetric and full products; INT_MAX behind the last
 };
 
 __device__ __forceinline__ int find(const Mats* __restrict__ t, int kind, int tile) {
   const bool behind = (threadIdx.x & 63) < kMats && t->first[kind][threadIdx.x & (kMats - 1)] <= tile;
   return __builtin_amdgcn_readfirstlane(__popcll(__ballot(behind)) - 1);
-}
-
-__global__ __launch_bounds__(256) void ns_table_kernel(const Mats t, Mats* __restrict__ table) {
-  for (int i = threadIdx.x; i < (int)(sizeof(Mats) / 4); i += 256) ((uint32_t*)table)[i] = ((const uint32_t*)&t)[i];
 }
 
 template <typename E>
@@ -104,7 +100,8 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const Mats t, Mats* __rest
   if (threadIdx.x == 0) M.norm[blockIdx.x] = v[0];
 }
 
-// element (r, k) of a factor with K (padded) columns: hi at the returned index, lo 32 behind it
+// element (r, k) of a factor with K (padded) columns: hi at the returned index, lo 32 behind it.  (Rows of an odd number of
+// 128-byte lines, so that one column's lines spread over more of the L2's channels, made no difference.)
 __device__ __forceinline__ int64_t at(int64_t r, int k, int K) { return (r * (K >> 5) + (k >> 5)) * 64 + (k & 31); }
 
 __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
@@ -161,7 +158,7 @@ struct Where {
 // The tile with this number in a launch.  Symmetric products count the tiles on and above the diagonal, row by row.
 template <int MODE, int T>
 __device__ __forceinline__ Where where(const Mats* __restrict__ t, int tile) {
-  constexpr int kind = MODE < NEXT ? SYM : FULL;
+  constexpr int kind = (MODE < NEXT ? SYM : FULL) + (T == 256 ? 2 : T == 128 ? 1 : 0);
   Where w;
   w.mat = find(t, kind, tile);
   const Mat& M = t->m[w.mat];
@@ -231,6 +228,59 @@ __device__ __forceinline__ void write_block(const Mat& M, int cur, const Coeffs&
   }
 }
 
+// Eight results (times 2^24) next to each other along a row of the product, ROW, or down a column, from (row, col) on, which
+// the mirrored or transposed factor holds along its row.
+template <int MODE, bool ROW, typename E>
+__device__ __forceinline__ void write8(const Mat& M, int cur, const Coeffs& f, const float (&sum)[8], int row, int col) {
+  const int r = ROW ? row : col, k = ROW ? col : row;    // row and first column where they are stored
+  if (MODE == LAST) {
+    if (r >= M.rows || k >= M.cols) return;
+    struct __attribute__((packed, aligned(sizeof(E)))) raw {
+      E v[8];
+    } v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.v[i] = (E)(sum[i] * (1.f / (kScale * kScale)));
+    E* o = (E*)M.out + (int64_t)r * M.cols + k;
+    if (k + 8 <= M.cols) {
+      *reinterpret_cast<raw*>(o) = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i < M.cols) o[i] = v.v[i];
+    }
+    return;
+  }
+  const int K = MODE == NEXT && ROW ? M.np : M.mp;
+  f16x8 hi, lo, ah, al;
+  if (MODE == POLY) {
+    const _Float16* p = M.a + at(r, k, K);
+    ah = *(const f16x8*)p, al = *(const f16x8*)(p + 32);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float v = sum[i] * (1.f / kScale);
+    if (MODE == POLY) {
+      v = fmaf(f.c, v, f.b * ((float)ah[i] + (float)al[i]));
+      if (r == k + i) v += f.a * kScale;
+    }
+    _Float16 vh, vl;
+    split(v, vh, vl);
+    hi[i] = vh, lo[i] = vl;
+  }
+  _Float16* o = (MODE == GRAM ? M.a : MODE == POLY ? M.q : ROW ? M.x : M.xt[cur ^ 1]) + at(r, k, K);
+  *(f16x8*)o = hi;
+  *(f16x8*)(o + 32) = lo;
+}
+// Which ways a tile is written.
+template <int MODE>
+__device__ __forceinline__ bool by_rows(const Mat& M) {
+  return MODE != LAST || !M.tall;
+}
+template <int MODE>
+__device__ __forceinline__ bool by_columns(const Mat& M, const Where& w) {
+  return MODE == NEXT || (MODE == LAST ? M.tall != 0 : w.tr != w.tc);
+}
+
 // This wave's loads but the last N have arrived and its reads of LDS are done; then the workgroup's barrier.  (__syncthreads
 // waits for all loads.)
 template <int N>
@@ -238,29 +288,35 @@ __device__ __forceinline__ void wait_and_sync() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// A workgroup's tile of T x T: waves, 32 x 32 blocks of a wave, LDS stages of 2 T rows x 128 bytes.  What bounds a stage is the
-// LDS: a wave reads its rows of both factors, the loads write them.  128: 64 + 32 KB a stage against 768 cycles of matrix pipe,
-// at 128 bytes a cycle all of it; 256: half of that per operation, but a matrix of 4096 has just one tile for
-// each CU.  64: for few tiles.
-// NS stages: two for 256 and 128.  64 x 64 tiles come where the chip is not full and a load's way from another XCD's
-// results (1 us) is what counts: 4, or 8 with one workgroup a CU.
-template <int T>
+// A workgroup's tile of T x T: waves, 32 x 32 blocks of a wave, NS LDS stages of 2 T rows x 128 bytes.
+// 256 and 128 (two stages): where the chip is full.  128 moves 96 KB through the LDS a stage, against 768 cycles of matrix
+// pipe, and twice 256's bytes from L2 per operation; but a matrix of 4096 has just one tile of 256 for each CU.
+// 64: for few tiles.  What counts then is the time of a stage on its own (reads of the LDS, then three dependent
+// products, twice: ~900 cycles) and a load's way from another XCD's results (1 us): four stages, and where one workgroup
+// has a CU for itself, G = 2 sets of four waves that take every other 32 columns and add up in the end (128: eight waves).
+template <int T, int G>
 struct Shape {
-  static constexpr int waves = T == 256 ? 8 : 4, cols = waves / 2;                   // 2 rows of waves
+  static constexpr int sets = T == 64 ? G : 1, waves = T == 256 ? 8 : T == 128 ? 4 * G : 4;         // waves of a set: 2 rows of
+  static constexpr int cols = waves / 2, threads = waves * sets * 64;
   static constexpr int nx = T / 64, ny = T / 32 / cols;
   static constexpr int passes = T / (8 * waves);                                     // load instructions of a wave per factor
 };
+constexpr int kPitch = 65;   // floats of a row of a 64 x 64 tile in LDS: rows and columns are read without conflicts
+
+// Where piece k of a row of 8 lies, and which piece lies at place k.  (The loads' row is taken within its pass of 8 x waves rows.)
+__device__ __forceinline__ int place(int row, int k) { return k ^ ((row >> 1) & 7); }
 
 // One T x T tile of P Q^T per workgroup, the factors loaded straight from memory to LDS.  The 16-byte pieces of an LDS row are
-// permuted by its row number, so that the 8 lanes that are served together read 8 different ones.
-// Tiles from `full` on are split along K into S slices of a workgroup each, whose sums go to `part`, 16 values of a lane
-// together, for ns_finish_kernel: the tiles that would make a round of their own on an idle chip.
-template <int MODE, int T, int NS, typename E>
-__global__ __launch_bounds__(Shape<T>::waves * 64) void ns_product_kernel(const Mats* __restrict__ t, int cur, Coeffs f,
-                                                                         int full, int S, float* __restrict__ part) {
-  typedef Shape<T> G;
-  constexpr int NX = G::nx, NY = G::ny, L = 2 * G::passes;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[NS][2][T * 128];
+// permuted (place()), so that the 16 lanes that a read serves together hit all 64 banks: 16 rows have 8 permutations, of
+// the even and of the odd ones, which are 128 bytes apart.  (Permuted by row & 7: half of all reads took 4 cycles more.)
+// Tiles from `full` on are split along K into S slices of a workgroup each, whose sums go to `part` for ns_finish_kernel: the
+// tiles that would make a round of their own on an idle chip.
+template <int MODE, int T, int G_, int NS, typename E>
+__global__ __launch_bounds__((Shape<T, G_>::threads)) void ns_product_kernel(const Mats* __restrict__ t, int cur, Coeffs f,
+                                                                          int full, int S, float* __restrict__ part) {
+  typedef Shape<T, G_> G;
+  constexpr int NX = G::nx, NY = G::ny, L = 2 * G::passes, KG = G::sets;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[NS][KG][2][T * 128];
   const int q = (int)blockIdx.x - full;
   const Where at_ = where<MODE, T>(t, q < 0 ? neighbours(blockIdx.x, full) : full + q / S);
   const Mat M = t->m[at_.mat];
@@ -269,20 +325,22 @@ __global__ __launch_bounds__(Shape<T>::waves * 64) void ns_product_kernel(const 
   const _Float16* P = MODE == GRAM ? M.x : MODE == POLY ? M.a : M.q;
   const _Float16* Q = MODE == GRAM ? M.x : MODE == POLY ? M.a : M.xt[cur];
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // a load instruction of a wave fills 1 KB = 8 rows; lane -> row l >> 3, piece (l & 7) ^ (row & 7)
+  const int set = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / G::waves;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - set * G::waves;
+  // a load instruction of a wave fills 1 KB = 8 rows; lane -> row l >> 3 of them, and the piece that belongs at its place
   const int64_t pitch = (int64_t)K * 4;   // bytes of a row
-  const uint8_t *src[2];
-  src[0] = (const uint8_t*)P + (int64_t)(tr * T + wave * 8 + (lane >> 3)) * pitch + ((lane & 7) ^ (lane >> 3)) * 16;
-  src[1] = (const uint8_t*)Q + (int64_t)(tc * T + wave * 8 + (lane >> 3)) * pitch + ((lane & 7) ^ (lane >> 3)) * 16;
+  const int lrow = wave * 8 + (lane >> 3), lpiece = place(lrow, lane & 7);
+  const uint8_t* src[2];
+  src[0] = (const uint8_t*)P + (int64_t)(tr * T + lrow) * pitch + set * 128 + lpiece * 16;
+  src[1] = (const uint8_t*)Q + (int64_t)(tc * T + lrow) * pitch + set * 128 + lpiece * 16;
   auto stage = [&](int s, int k) {
 #pragma unroll
     for (int o = 0; o < 2; ++o)
 #pragma unroll
       for (int j = 0; j < G::passes; ++j)
         __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)(src[o] + (int64_t)(8 * G::waves * j) * pitch + (int64_t)k * 128),
-            (__attribute__((address_space(3))) void*)(&lds[s][o][(8 * G::waves * j + wave * 8) * 128]), 16, 0, 0);
+            (const __attribute__((address_space(1))) void*)(src[o] + (int64_t)(8 * G::waves * j) * pitch + (int64_t)k * (KG * 128)),
+            (__attribute__((address_space(3))) void*)(&lds[s][set][o][(8 * G::waves * j + wave * 8) * 128]), 16, 0, 0);
   };
   f32x16 acc[NX][NY];
 #pragma unroll
@@ -292,7 +350,7 @@ __global__ __launch_bounds__(Shape<T>::waves * 64) void ns_product_kernel(const 
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
   const int wr = wave / G::cols * (32 * NX), wc = wave % G::cols * (32 * NY);
-  const int steps = K / kBK;
+  const int steps = K / (kBK * KG);     // (K is a multiple of 64)
   const int slice = q < 0 ? 0 : q % S;
   const int begin = q < 0 ? 0 : (int)((int64_t)steps * slice / S);
   const int end = q < 0 ? steps : (int)((int64_t)steps * (slice + 1) / S);
@@ -305,12 +363,10 @@ __global__ __launch_bounds__(Shape<T>::waves * 64) void ns_product_kernel(const 
     const int behind = end - 1 - k;
     if (NS == 2 || behind == 0) wait_and_sync<0>();
     else if (behind >= NS - 2) wait_and_sync<(NS - 2) * L>();
-    else if (NS > 4 && behind >= 4) wait_and_sync<4 * L>();
-    else if (NS > 4 && behind >= 2) wait_and_sync<2 * L>();
     else wait_and_sync<L>();
     if (k + NS - 1 < end) stage(s == 0 ? NS - 1 : s - 1, k + NS - 1);
-    const uint8_t* lp = lds[s][0];
-    const uint8_t* lq = lds[s][1];
+    const uint8_t* lp = lds[s][set][0];
+    const uint8_t* lq = lds[s][set][1];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {      // 16 columns
       f16x8 ph[NX], pl[NX], qh[NY], ql[NY];
@@ -318,14 +374,14 @@ __global__ __launch_bounds__(Shape<T>::waves * 64) void ns_product_kernel(const 
 #pragma unroll
       for (int x = 0; x < NX; ++x) {
         const int r = wr + 32 * x + (lane & 31);
-        ph[x] = *(const f16x8*)(lp + r * 128 + (piece ^ (r & 7)) * 16);
-        pl[x] = *(const f16x8*)(lp + r * 128 + ((piece + 4) ^ (r & 7)) * 16);
+        ph[x] = *(const f16x8*)(lp + r * 128 + place(r, piece) * 16);
+        pl[x] = *(const f16x8*)(lp + r * 128 + place(r, piece + 4) * 16);
       }
 #pragma unroll
       for (int y = 0; y < NY; ++y) {
         const int r = wc + 32 * y + (lane & 31);
-        qh[y] = *(const f16x8*)(lq + r * 128 + (piece ^ (r & 7)) * 16);
-        ql[y] = *(const f16x8*)(lq + r * 128 + ((piece + 4) ^ (r & 7)) * 16);
+        qh[y] = *(const f16x8*)(lq + r * 128 + place(r, piece) * 16);
+        ql[y] = *(const f16x8*)(lq + r * 128 + place(r, piece + 4) * 16);
       }
 #pragma unroll
       for (int x = 0; x < NX; ++x)
@@ -341,20 +397,57 @@ __global__ __launch_bounds__(Shape<T>::waves * 64) void ns_product_kernel(const 
         for (int y = 0; y < NY; ++y) acc[x][y] = mfma(ph[x], qh[y], acc[x][y]);
     }
   }
+  if constexpr (T == 64) {     // through LDS, to rows and columns of 8
+    static_assert(NS * 2 * T * 128 >= T * kPitch * (int)sizeof(float), "the sets' sums fit the stages");
+    float* tile = (float*)&lds[0][0][0][0];
+    __syncthreads();
 #pragma unroll
-  for (int x = 0; x < NX; ++x)
+    for (int r = 0; r < 16; ++r)
+      tile[set * (T * kPitch) + (wr + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * kPitch + wc + (lane & 31)] = acc[0][0][r];
+    __syncthreads();
+    const bool rows = by_rows<MODE>(M), columns = by_columns<MODE>(M, at_);
+    for (int i = threadIdx.x; i < T * T / 8; i += G::threads) {
+      const int a = i >> 3, b = (i & 7) * 8;
+      float v[8];
+      if (rows || q >= 0) {
 #pragma unroll
-    for (int y = 0; y < NY; ++y) {
-      if (q < 0) {
-        write_block<MODE, E>(M, cur, f, acc[x][y], tr * T + wr + 32 * x, tc * T + wc + 32 * y, MODE >= NEXT || tr != tc);
-      } else {
-        const int block = (wr / 32 + x) * (T / 32) + wc / 32 + y;
-        *(f32x16*)(part + (((int64_t)(q / S) * (T / 32) * (T / 32) + block) * S + slice) * 1024 + lane * 16) = acc[x][y];
+        for (int j = 0; j < 8; ++j) {
+          v[j] = tile[a * kPitch + b + j];
+          if (KG == 2) v[j] += tile[T * kPitch + a * kPitch + b + j];
+        }
+        if (q < 0) {
+          write8<MODE, true, E>(M, cur, f, v, tr * T + a, tc * T + b);
+        } else {
+          float4* o = (float4*)(part + ((int64_t)(q / S) * S + slice) * (T * T) + a * T + b);
+          o[0] = float4{v[0], v[1], v[2], v[3]};
+          o[1] = float4{v[4], v[5], v[6], v[7]};
+        }
+      }
+      if (columns && q < 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[j] = tile[(b + j) * kPitch + a];
+          if (KG == 2) v[j] += tile[T * kPitch + (b + j) * kPitch + a];
+        }
+        write8<MODE, false, E>(M, cur, f, v, tr * T + b, tc * T + a);
       }
     }
+  } else {
+#pragma unroll
+    for (int x = 0; x < NX; ++x)
+#pragma unroll
+      for (int y = 0; y < NY; ++y) {
+        if (q < 0) {
+          write_block<MODE, E>(M, cur, f, acc[x][y], tr * T + wr + 32 * x, tc * T + wc + 32 * y, MODE >= NEXT || tr != tc);
+        } else {     // 16 values of a lane together
+          const int block = (wr / 32 + x) * (T / 32) + wc / 32 + y;
+          *(f32x16*)(part + (((int64_t)(q / S) * (T / 32) * (T / 32) + block) * S + slice) * 1024 + lane * 16) = acc[x][y];
+        }
+      }
+  }
 }
 
-// Adds the slices of the split tiles, in order: one wave per 32 x 32 block.
+// Adds the slices of the split tiles, in order: a wave per 32 x 32 block of T = 256 and 128,
 template <int MODE, int T, typename E>
 __global__ __launch_bounds__(64) void ns_finish_kernel(const Mats* __restrict__ t, int cur, Coeffs f, int full, int S,
                                                        const float* __restrict__ part) {
@@ -369,6 +462,35 @@ __global__ __launch_bounds__(64) void ns_finish_kernel(const Mats* __restrict__ 
   for (int k = 0; k < S; ++k) acc += *(const f32x16*)(p + (int64_t)k * 1024);
   write_block<MODE, E>(t->m[w.mat], cur, f, acc, w.tr * T + block / N * 32, w.tc * T + block % N * 32,
                        MODE >= NEXT || w.tr != w.tc);
+}
+
+// and 16 rows of a 64 x 64 tile by a workgroup of two waves.
+template <int MODE, typename E>
+__global__ __launch_bounds__(128) void ns_finish64_kernel(const Mats* __restrict__ t, int cur, Coeffs f, int full, int S,
+                                                          const float* __restrict__ part) {
+  constexpr int T = 64, R = 16;
+  __shared__ float tile[R][kPitch];
+  const int split = blockIdx.x / (T / R), band = blockIdx.x % (T / R);
+  const Where w = where<MODE, T>(t, full + split);
+  const Mat M = t->m[w.mat];
+  const int a = threadIdx.x >> 3, b = (threadIdx.x & 7) * 8;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const float* p = part + (int64_t)split * S * (T * T) + (band * R + a) * T + b;
+#pragma unroll 4
+  for (int k = 0; k < S; ++k) {
+    const float4 x = *(const float4*)(p + (int64_t)k * (T * T)), y = *(const float4*)(p + (int64_t)k * (T * T) + 4);
+    v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+    v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+  }
+  if (by_rows<MODE>(M)) write8<MODE, true, E>(M, cur, f, v, w.tr * T + band * R + a, w.tc * T + b);
+  if (!by_columns<MODE>(M, w)) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) tile[a][b + j] = v[j];
+  __syncthreads();
+  const int col = threadIdx.x >> 1, r0 = (threadIdx.x & 1) * 8;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = tile[r0 + j][col];
+  write8<MODE, false, E>(M, cur, f, v, w.tr * T + band * R + r0, w.tc * T + col);
 }
 
 // ------------------------------------------------------------------------------------ host side
@@ -393,85 +515,99 @@ struct List {
   int place[kMats];   // in the caller's list
 };
 
+// The shapes that a product is compiled for.  per_cu: workgroups that a CU holds (LDS); stage: us of a stage of 32 columns
+// where nothing else bounds it, as measured.
+struct Variant {
+  int T, G, per_cu;
+  double stage;
+};
+constexpr Variant kVariants[] = {{64, 2, 1, 0.27}, {64, 1, 2, 0.42}, {128, 2, 1, 0.95}, {128, 1, 2, 1.2}, {256, 1, 1, 2.85}};
+
 // How a product of all matrices is launched.
 struct Launch {
-  int T;            // tile side
+  Variant v;
   int tiles, full;  // tiles, and how many of them are not split
   int S;            // slices of the others
-  double cost;      // in rounds of 128 x 128 tiles
+  double us;        // estimated
   int groups() const { return full + (tiles - full) * S; }
-  int64_t part_floats() const { return (int64_t)(tiles - full) * S * T * T; }
+  int64_t part_floats() const { return (int64_t)(tiles - full) * S * v.T * v.T; }
 };
 
-// The workgroups that the chip holds at a time (2 a CU, of T = 256 one) make a round.  The tiles of whole rounds are not
-// split.  Those left over are, where they would leave two thirds of the chip idle: into as many slices as the chip has
-// room for, of at least 12 stages.
-Launch launch_with(const List& l, int mode, int T) {
-  Launch r = {T, 0, 0, 1, 0.0};
-  int64_t tiles = 0, steps = 0;
+// The workgroups that the chip holds at a time make a round.  Tiles of whole rounds are not split; those left over may be,
+// into slices of at least 8 stages, where their sums' way through memory costs less than an idle chip.  A stage takes the
+// variant's time or what the loads of all CUs need for its bytes (measured: 8.7 TB/s, from 128 x 128 tiles on 10.8); a launch
+// has 3.5 us around its stages, and a second round on CUs that hold one workgroup 2.5 of its own.
+Launch launch_with(const List& l, int mode, const Variant& v) {
+  double work = 0.0;
+  int64_t tiles = 0, longest = 0;
   for (int i = 0; i < l.n; ++i) {
-    tiles += tiles_of(l.t.m[i], mode < NEXT, T);
-    steps = std::max<int64_t>(steps, (mode == GRAM ? l.t.m[i].np : l.t.m[i].mp) / kBK);
+    const int64_t n = tiles_of(l.t.m[i], mode < NEXT, v.T), steps = (mode == GRAM ? l.t.m[i].np : l.t.m[i].mp) / kBK;
+    tiles += n;
+    work += (double)n * steps;
+    longest = std::max(longest, steps);
   }
-  const int64_t round = (T == 256 ? 1 : 2) * kCUs, rest = tiles % round;
-  r.tiles = r.full = (int)tiles;
-  int64_t S = rest ? std::min(round / rest, steps / 12) : 1;
-  if (S > 8) S &= ~7;               // slice k of all tiles on XCD k mod 8: each reads its columns only
-  if (S >= 3) r.full = (int)(tiles - rest), r.S = (int)S;
-  r.cost = (double)(tiles / round) + (rest ? (S >= 3 ? 0.1 + 1.0 / S : 1.0) : 0.0);
-  if (T == 256) r.cost *= 1.7;      // (4 times the tile, by twice the waves: 2 at the same rate)
+  const int64_t round = (int64_t)v.per_cu * kCUs, rest = tiles % round, full = tiles - rest;
+  const double average = work / tiles;
+  auto stage = [&](int64_t groups) {
+    return std::max(v.stage, (double)std::min(groups, round) * v.T * 256 / (v.T == 64 ? 8.7e6 : 10.8e6));
+  };
+  const double rounds = (double)(full / round), own = v.per_cu == 1 ? 2.5 : 0.0;
+  const double whole = full ? rounds * average * stage(full) + (rounds - (rest ? 0 : 1)) * own : 0.0;
+  Launch r = {v, (int)tiles, (int)tiles, 1, 3.5 + whole + (rest ? longest * stage(rest) : 0.0)};
+  for (int64_t S = 2; rest && S <= std::min<int64_t>(round / rest, longest / 8); S += S < 8 ? 1 : 8) {   // (from 8 on by 8: slice k
+    // of all tiles on XCD k mod 8, which reads its columns only)
+    const double us = 3.5 + whole + (double)longest / S * stage(rest * S) + 4.5 + rest * S * v.T * v.T * 8 / 4e6;
+    if (us < r.us) r.full = (int)full, r.S = (int)S, r.us = us;
+  }
   return r;
 }
 
 Launch launch_of(const List& l, int mode) {
-  if (l.unit == 64) return launch_with(l, mode, 64);
-  const Launch r = launch_with(l, mode, 128);
-  if (l.unit == 128) return r;
-  const Launch q = launch_with(l, mode, 256);
-  return q.cost < r.cost ? q : r;
+  Launch best = {};
+  for (const Variant& v : kVariants) {
+    if (v.T > l.unit) continue;
+    const Launch r = launch_with(l, mode, v);
+    if (best.tiles == 0 || r.us < best.us) best = r;
+  }
+  return best;
 }
 
-template <int MODE, int T, int NS, typename E>
+template <int MODE, int T, int G, int NS, typename E>
 void product_with(const Launch& r, const Mats* t, int cur, const Coeffs& f, float* part, hipStream_t s) {
-  RL_LAUNCH((ns_product_kernel<MODE, T, NS, E>), dim3((unsigned)r.groups()), dim3(Shape<T>::waves * 64), 0, s, t, cur, f,
+  RL_LAUNCH((ns_product_kernel<MODE, T, G, NS, E>), dim3((unsigned)r.groups()), dim3(Shape<T, G>::threads), 0, s, t, cur, f,
             r.full, r.S, part);
-  if (r.tiles > r.full)
-    RL_LAUNCH((ns_finish_kernel<MODE, T, E>), dim3((unsigned)((r.tiles - r.full) * (T / 32) * (T / 32))), dim3(64), 0, s, t,
-              cur, f, r.full, r.S, part);
+  const int split = r.tiles - r.full;
+  if (split == 0) return;
+  if constexpr (T == 64)
+    RL_LAUNCH((ns_finish64_kernel<MODE, E>), dim3((unsigned)(split * 4)), dim3(128), 0, s, t, cur, f, r.full, r.S, part);
+  else
+    RL_LAUNCH((ns_finish_kernel<MODE, T, E>), dim3((unsigned)(split * (T / 32) * (T / 32))), dim3(64), 0, s, t, cur, f,
+              r.full, r.S, part);
 }
 
-// `first` of the table counts tiles of one side: a launch of 256 x 256 tiles takes the second table
 template <int MODE, typename E>
 void product(const List& l, const Mats* table, int cur, const Coeffs& f, float* part, hipStream_t s) {
   const Launch r = launch_of(l, MODE);
-  if (r.T == 256) product_with<MODE, 256, 2, E>(r, table + 1, cur, f, part, s);
-  else if (r.T == 128) product_with<MODE, 128, 2, E>(r, table, cur, f, part, s);
-  else if (r.groups() > kCUs) product_with<MODE, 64, 4, E>(r, table, cur, f, part, s);
-  else product_with<MODE, 64, 8, E>(r, table, cur, f, part, s);
-}
-
-void number_tiles(List& l, int T) {
-  int sum[3] = {0, 0, 0};
-  for (int i = 0; i < kMats; ++i) {
-    for (int k = 0; k < 3; ++k) l.t.first[k][i] = i < l.n ? sum[k] : INT_MAX;
-    if (i >= l.n) continue;
-    sum[LOAD] += (l.t.m[i].mp / 32) * (l.t.m[i].np / 32);
-    sum[SYM] += (int)tiles_of(l.t.m[i], true, T);
-    sum[FULL] += (int)tiles_of(l.t.m[i], false, T);
-  }
+  if (r.v.T == 256) product_with<MODE, 256, 1, 2, E>(r, table, cur, f, part, s);
+  else if (r.v.T == 128 && r.v.G == 1) product_with<MODE, 128, 1, 2, E>(r, table, cur, f, part, s);
+  else if (r.v.T == 128) product_with<MODE, 128, 2, 4, E>(r, table, cur, f, part, s);
+  else if (r.v.G == 1) product_with<MODE, 64, 1, 4, E>(r, table, cur, f, part, s);
+  else product_with<MODE, 64, 2, 4, E>(r, table, cur, f, part, s);
 }
 
 template <typename E>
 int run(List& l, int steps, const Coeffs& f, double eps, Mats* table, float* part, hipStream_t s) {
-  int tiles = 0;
-  for (int i = 0; i < l.n; ++i) tiles += (l.t.m[i].mp / 32) * (l.t.m[i].np / 32);
-  if (l.unit == 256) {
-    number_tiles(l, 256);
-    RL_LAUNCH((ns_table_kernel), dim3(1), dim3(256), 0, s, l.t, table + 1);
+  int64_t sum[KINDS] = {};
+  for (int i = 0; i < kMats; ++i) {
+    for (int k = 0; k < KINDS; ++k) l.t.first[k][i] = i < l.n ? (int)sum[k] : INT_MAX;
+    if (i >= l.n) continue;
+    const Mat& m = l.t.m[i];
+    sum[LOAD] += (int64_t)(m.mp / 32) * (m.np / 32);
+    for (int k = 0; k < 3 && (64 << k) <= l.unit; ++k)
+      sum[SYM + k] += tiles_of(m, true, 64 << k), sum[FULL + k] += tiles_of(m, false, 64 << k);
   }
-  number_tiles(l, l.unit == 64 ? 64 : 128);
   RL_LAUNCH((ns_norm_kernel<E>), dim3(kNormBlocks, l.n), dim3(256), 0, s, l.t, table);
-  RL_LAUNCH((ns_load_kernel<E>), dim3((unsigned)tiles), dim3(256), 0, s, table, eps);
+  RL_LAUNCH((ns_load_kernel<E>), dim3((unsigned)sum[LOAD]), dim3(256), 0, s, table, eps);
   for (int k = 0; k < steps; ++k) {
     product<GRAM, float>(l, table, 0, f, part, s);
     product<POLY, float>(l, table, 0, f, part, s);
@@ -482,9 +618,8 @@ int run(List& l, int steps, const Coeffs& f, double eps, Mats* table, float* par
   return RLPYT_OK;
 }
 
-// The matrices lo .. of a list that go together (at most kMats, empty ones left out) and what their sides are padded to;
-// -> where the next ones start.  64 where 128 x 128 tiles would be too few for the chip, 256 where 256 x 256 ones are enough
-// and the larger pads cost less than those tiles gain.
+// The matrices lo .. of a list that go together (at most kMats, empty ones left out) and what their sides are padded to, 64,
+// 128 or 256: what is expected to take the least time, with the tiles that this allows; -> where the next ones start.
 int gather(const int64_t* rows, const int64_t* cols, int n, int lo, List& l) {
   l.n = 0;
   for (; lo < n && l.n < kMats; ++lo) {
@@ -495,19 +630,22 @@ int gather(const int64_t* rows, const int64_t* cols, int n, int lo, List& l) {
     m.rows = (int)rows[lo], m.cols = (int)cols[lo];
     m.tall = m.rows > m.cols;
   }
-  auto pads = [&](int unit) {
+  if (l.n == 0) return lo;
+  auto with = [&](int unit) {
     l.unit = unit;
-    int64_t sum = 0;
     for (int i = 0; i < l.n; ++i) {
       Mat& m = l.t.m[i];
       m.mp = pad(std::min(m.rows, m.cols), unit), m.np = pad(std::max(m.rows, m.cols), unit);
-      sum += (int64_t)m.mp * m.np;
     }
-    return sum;
+    return launch_of(l, GRAM).us + launch_of(l, POLY).us + launch_of(l, NEXT).us;
   };
-  const int64_t wide = pads(256), usual = pads(128);
-  if (usual < (int64_t)kCUs * 128 * 128) pads(64);
-  else if (wide >= (int64_t)kCUs * 256 * 256 && wide < usual + usual / 16) pads(256);
+  int unit = 64;
+  double least = with(64);
+  for (int u : {128, 256}) {
+    const double us = with(u);
+    if (us < least) least = us, unit = u;
+  }
+  with(unit);
   return lo;
 }
 
@@ -517,9 +655,9 @@ int64_t part_floats(const List& l) {
   return most;
 }
 
-// workspace: two tables | sums of slices | the matrices' factors
-constexpr int64_t kTables = 2 * sizeof(Mats);
-static_assert(sizeof(Mats) % 16 == 0 && sizeof(Mats) + 16 <= 4096, "an argument, and aligned pieces behind two of them");
+// workspace: table | sums of slices | the matrices' factors
+constexpr int64_t kTables = sizeof(Mats);
+static_assert(sizeof(Mats) % 16 == 0 && sizeof(Mats) + 16 <= 4096, "an argument, and aligned pieces behind it");
 
 }  // namespace
 }  // namespace rlpyt
