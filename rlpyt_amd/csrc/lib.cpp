@@ -120,7 +120,12 @@ extern "C" int rlpyt_hip_device_info(char* name, int cap) {
 
 extern "C" int rlpyt_host_register(void* host_ptr, int64_t bytes) {
   RL_CHECK_ARG(host_ptr != nullptr && bytes > 0, RLPYT_EINVAL, "rlpyt_host_register: bad range");
-  RL_HIP(hipHostRegister(host_ptr, (size_t)bytes, hipHostRegisterPortable | hipHostRegisterMapped));
+  const hipError_t e = hipHostRegister(host_ptr, (size_t)bytes, hipHostRegisterPortable | hipHostRegisterMapped);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();   // the caller falls back to pageable copies: its next HIP call must not report this one
+    rlpyt::set_error("hipHostRegister of %ld bytes failed: %s", (long)bytes, hipGetErrorString(e));
+    return RLPYT_EHIP;
+  }
   return RLPYT_OK;
 }
 
