@@ -860,19 +860,20 @@ int rlpyt_gated_scan_step(int dtype, const void* x, int64_t x_bs, const void* ga
  *   r = exp(logp - old_logp)    pi = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)    d = ref_logp - logp
  *   loss = sum valid (pi + kl_coeff (e^d - d - 1) - entropy_coeff H) / sum valid
  * ref_logp, valid (f32 weights; rows of weight 0 are not read) may be null.  scalars [5] = loss (also
- * in *loss), pi, kl, entropy and clipped share (weighted means; 0 when nothing is valid).  grad [N,V] dense (may be null): d loss / d logits.  A row of -inf only adds nothing; an action
+ * in *loss), pi, kl, entropy and clipped share (weighted means; 0 when nothing is valid).  grad [N,V] dense (may be null): grad_scale d loss /
+ * d logits.  A row of -inf only adds nothing; an action
  * outside 0 .. V-1 makes the loss NaN. */
 int64_t rlpyt_policy_loss_workspace_bytes(int dtype, int64_t N, int64_t V);
 int rlpyt_policy_kl_loss_fwd_bwd(int dtype, const void* logits, int64_t row_stride, const int64_t* action,
                                  const float* old_logp, const float* advantage, const float* ref_logp,
                                  const float* valid, int64_t N, int64_t V, double clip_low, double clip_high,
-                                 double kl_coeff, double entropy_coeff, float* loss, float* scalars,
-                                 void* grad, void* workspace, rlpyt_stream_t stream);
+                                 double kl_coeff, double entropy_coeff, double grad_scale, float* loss,
+                                 float* scalars, void* grad, void* workspace, rlpyt_stream_t stream);
 /* log softmax(logits)[action] and the entropy of every row. */
 int rlpyt_action_logp(int dtype, const void* logits, int64_t row_stride, const int64_t* action, int64_t N,
                       int64_t V, float* logp, float* entropy, void* workspace, rlpyt_stream_t stream);
-/* x *= *scale in place (x 16-byte aligned); nothing is touched where the device scalar is 1. */
-int rlpyt_scale_unless_one(int dtype, void* x, int64_t n, const float* scale, rlpyt_stream_t stream);
+/* x *= *scale * factor in place (x 16-byte aligned, *scale on the device); nothing is touched where that is 1. */
+int rlpyt_scale_unless_one(int dtype, void* x, int64_t n, const float* scale, float factor, rlpyt_stream_t stream);
 
 /* Newton-Schulz orthogonalisation of n matrices (host tables; matrix i is rows[i] x cols[i], row stride ld[i],
  * its result dense):  X = G / (|G|_F + eps),  steps x:  X <- a X + (b A + c A A) X  with  A = X X^T (of the wide

@@ -218,9 +218,9 @@ _SIGNATURES = {
     "rlpyt_gated_scan_step": (c_int, [c_int, _p, c_int64, _p, c_int64, _p, _p, _p, c_int64, c_int64, _p]),
     "rlpyt_policy_loss_workspace_bytes": (c_int64, [c_int, c_int64, c_int64]),
     "rlpyt_policy_kl_loss_fwd_bwd": (c_int, [c_int, _p, c_int64, _p, _p, _p, _p, _p, c_int64, c_int64, c_double,
-                                             c_double, c_double, c_double, _p, _p, _p, _p, _p]),
+                                             c_double, c_double, c_double, c_double, _p, _p, _p, _p, _p]),
     "rlpyt_action_logp": (c_int, [c_int, _p, c_int64, _p, c_int64, c_int64, _p, _p, _p, _p]),
-    "rlpyt_scale_unless_one": (c_int, [c_int, _p, c_int64, _p, _p]),
+    "rlpyt_scale_unless_one": (c_int, [c_int, _p, c_int64, _p, c_float, _p]),
     "rlpyt_orthogonalize_workspace_bytes": (c_int64, [_p, _p, c_int]),
     "rlpyt_orthogonalize": (c_int, [c_int, _p, _p, _p, _p, _p, c_int, c_int, c_float, c_float, c_float, c_double,
                                     _p, _p]),

@@ -43,7 +43,7 @@ struct LossArgs {
   float3* parts;                  // split rows: (max, sum, weighted sum) of the parts [N, P]
   int64_t N, n0, n_rows;          // a launch takes the rows n0 .. n0 + n_rows - 1
   int V, part;                    // part: elements of a row's part, a multiple of 8
-  double lo, hi, c_kl, c_ent;
+  double lo, hi, c_kl, c_ent, g_scale;
 };
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -137,7 +137,7 @@ __device__ __forceinline__ RowOut row_terms(const LossArgs& p, int64_t n, float 
   }
   o.ent = H;
   const double denom = p.denom ? *p.denom : (double)p.N;
-  const double g = denom > 0.0 ? (double)w / denom : 0.0, gs = g / (double)st.s;
+  const double g = denom > 0.0 ? p.g_scale * (double)w / denom : 0.0, gs = g / (double)st.s;
   o.k1 = (float)(gs * p.c_ent * kLn2);
   o.k0 = (float)(gs * (p.c_ent * (H - logs) - c));
   o.ka = (float)(g * c);
@@ -484,13 +484,13 @@ __global__ __launch_bounds__(1024) void loss_finish_kernel(const double* __restr
   for (int k = 0; k < 4; ++k) scalars[1 + k] = (float)v[k];
 }
 
-// grad *= *scale, in place; nothing is read or written where *scale is 1 (hence a grid that the chip holds at once).
+// grad *= *scale * factor, in place; nothing is read or written where that is 1 (hence a grid that the chip holds at once).
 template <typename E>
 __global__ __launch_bounds__(256) void loss_scale_kernel(E* __restrict__ g, int64_t n,
-                                                         const float* __restrict__ scale) {
+                                                         const float* __restrict__ scale, float factor) {
   typedef typename Row16<E>::vec vec;
   constexpr int n16 = Row16<E>::n;
-  const float f = *scale;
+  const float f = *scale * factor;
   if (f == 1.f) return;
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * n16; i < n; i += (int64_t)gridDim.x * 256 * n16) {
     if (i + n16 <= n) {
@@ -604,8 +604,8 @@ extern "C" int rlpyt_policy_kl_loss_fwd_bwd(int dtype, const void* logits, int64
                                             const int64_t* action, const float* old_logp,
                                             const float* advantage, const float* ref_logp, const float* valid,
                                             int64_t N, int64_t V, double clip_low, double clip_high,
-                                            double kl_coeff, double entropy_coeff, float* loss, float* scalars,
-                                            void* grad, void* workspace, rlpyt_stream_t stream) {
+                                            double kl_coeff, double entropy_coeff, double grad_scale, float* loss,
+                                            float* scalars, void* grad, void* workspace, rlpyt_stream_t stream) {
   RL_CHECK_ARG(dtype >= F32 && dtype <= F16, RLPYT_EINVAL, "rlpyt_policy_kl_loss_fwd_bwd: unknown dtype %d", dtype);
   RL_CHECK_ARG(N >= 0 && V > 0 && V <= (1 << 30), RLPYT_ESHAPE,
                "rlpyt_policy_kl_loss_fwd_bwd: N=%ld V=%ld out of range", (long)N, (long)V);
@@ -622,7 +622,7 @@ extern "C" int rlpyt_policy_kl_loss_fwd_bwd(int dtype, const void* logits, int64
   p.denom = valid ? denom : nullptr;
   p.parts = (float3*)((char*)workspace + parts_offset(q));
   p.N = N, p.V = (int)V, p.part = q.part;
-  p.lo = clip_low, p.hi = clip_high, p.c_kl = kl_coeff, p.c_ent = entropy_coeff;
+  p.lo = clip_low, p.hi = clip_high, p.c_kl = kl_coeff, p.c_ent = entropy_coeff, p.g_scale = grad_scale;
   if (valid) RL_LAUNCH(loss_denom_kernel, dim3(1), dim3(1024), 0, s, valid, N, denom);
   const int rc = run_all(dtype, p, q, s);
   if (rc != RLPYT_OK) return rc;
@@ -648,7 +648,8 @@ extern "C" int rlpyt_action_logp(int dtype, const void* logits, int64_t row_stri
   return run_all(dtype, p, q, (hipStream_t)stream);
 }
 
-extern "C" int rlpyt_scale_unless_one(int dtype, void* x, int64_t n, const float* scale, rlpyt_stream_t stream) {
+extern "C" int rlpyt_scale_unless_one(int dtype, void* x, int64_t n, const float* scale, float factor,
+                                      rlpyt_stream_t stream) {
   RL_CHECK_ARG(dtype >= F32 && dtype <= F16, RLPYT_EINVAL, "rlpyt_scale_unless_one: unknown dtype %d", dtype);
   RL_CHECK_ARG(n >= 0, RLPYT_ESHAPE, "rlpyt_scale_unless_one: n=%ld out of range", (long)n);
   if (n == 0) return RLPYT_OK;
@@ -657,9 +658,9 @@ extern "C" int rlpyt_scale_unless_one(int dtype, void* x, int64_t n, const float
   hipStream_t s = (hipStream_t)stream;
   const int per = 256 * (16 / element_size(dtype));
   const dim3 grid((unsigned)std::min<int64_t>(1024, ceil_div(n, per)));
-  if (dtype == F32) RL_LAUNCH((loss_scale_kernel<float>), grid, dim3(256), 0, s, (float*)x, n, scale);
-  else if (dtype == BF16) RL_LAUNCH((loss_scale_kernel<__bf16>), grid, dim3(256), 0, s, (__bf16*)x, n, scale);
-  else RL_LAUNCH((loss_scale_kernel<_Float16>), grid, dim3(256), 0, s, (_Float16*)x, n, scale);
+  if (dtype == F32) RL_LAUNCH((loss_scale_kernel<float>), grid, dim3(256), 0, s, (float*)x, n, scale, factor);
+  else if (dtype == BF16) RL_LAUNCH((loss_scale_kernel<__bf16>), grid, dim3(256), 0, s, (__bf16*)x, n, scale, factor);
+  else RL_LAUNCH((loss_scale_kernel<_Float16>), grid, dim3(256), 0, s, (_Float16*)x, n, scale, factor);
   RL_LAUNCH_CHECK();
   return RLPYT_OK;
 }

@@ -8,7 +8,8 @@ the C ABI (``include/rlpyt_hip.h``); ``rlpyt_amd.ops`` offers them with the othe
 * ``orthogonalize``: the Newton-Schulz products behind ``rlpyt_amd.optim.Muon``.
 
 Arguments that do not fit raise ``ValueError`` before anything is launched.  Kernels run on the current stream of the
-tensors' device; workspaces come from torch's allocator per call, so that captured graphs do not share them.
+tensors' device; workspaces come from torch's allocator per call, so that captured graphs do not share them.  Behind the
+checks, the first four run in a small extension (``csrc/seqops.cpp``): allocations, launches and autograd nodes.
 """
 import ctypes
 
@@ -17,11 +18,19 @@ import torch
 from . import _lib
 from ._lib import check, lib
 
+try:
+    from . import _seqops       # (after _lib: it takes the C entry points from the library that is loaded there)
+except ImportError as e:
+    raise _lib.HipExtensionMissing(
+        f"rlpyt_amd/_seqops.so cannot be loaded ({e}). Run `python -c 'import __graft_entry__ as g; g.build()'` (or "
+        "`make -C rlpyt_amd/csrc`).") from e
+if _seqops.abi_version != _lib.ABI_VERSION:
+    raise _lib.HipExtensionMissing(
+        f"rlpyt_amd/_seqops.so has ABI {_seqops.abi_version}, binding expects {_lib.ABI_VERSION}: rebuild.")
+
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _FLOATS = (torch.float32, torch.float64, torch.bfloat16, torch.float16)
 _BYTES = (torch.bool, torch.uint8)
-# (torch.cuda.current_stream() builds a Stream object, 1 - 3 us a call; small calls here take 10)
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _refuse(text):
@@ -38,112 +47,9 @@ def _need_device(name, first, *others):
             _refuse(f"{name}: tensors on one device are needed, got {device} and {t.device}")
 
 
-def _p(t):
-    return None if t is None else t.data_ptr()
-
-
-def _launch(index, fn, *args):
-    """``fn(*args, stream)`` on device ``index`` and its current stream."""
-    if torch._C._cuda_getDevice() == index:
-        rc = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
-    if rc:
-        check(rc, fn.__name__)
-
-
-def _bytes(n, device):
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
-
-
-def _backward(fast):
-    """A backward pass that is not differentiable itself: the check costs 8 us, and is needed only where a graph
-    of the backward pass is built (gradients are enabled inside it then)."""
-    checked = torch.autograd.function.once_differentiable(fast)
-
-    def backward(ctx, *grads):
-        return checked(ctx, *grads) if torch.is_grad_enabled() else fast(ctx, *grads)
-
-    return staticmethod(backward)
-
-
 # --------------------------------------------------------------------------------------
 # gated linear recurrence
 # --------------------------------------------------------------------------------------
-def _unit_rows(t):
-    """``t`` with unit stride along its last axis."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-def _like_rows(x):
-    """An empty ``[T, B, D]`` whose rows lie in memory in the order of ``x``'s: time or batch first."""
-    if x.is_contiguous():
-        return torch.empty_like(x)
-    T, B, D = x.shape
-    if T > 1 and B > 1 and x.stride(1) > x.stride(0):
-        return torch.empty((B, T, D), dtype=x.dtype, device=x.device).transpose(0, 1)
-    return torch.empty((T, B, D), dtype=x.dtype, device=x.device)
-
-
-def _scan_forward(x, gate, h0, reset, lengths, keep):
-    T, B, D = x.shape
-    device = x.device
-    h = _like_rows(x)
-    hn = torch.empty((B, D), dtype=torch.float32, device=device)
-    states = (torch.empty((lib.rlpyt_gated_scan_state_rows(T), B, D), dtype=torch.float32, device=device)
-              if keep else None)
-    ws = _bytes(lib.rlpyt_gated_scan_workspace_bytes(T, B, D), device)
-    _launch(device.index, lib.rlpyt_gated_scan_fwd, _DTYPES[x.dtype], x.data_ptr(), *x.stride()[:2],
-            gate.data_ptr(), *gate.stride()[:2], _p(h0), _p(reset), _p(lengths), h.data_ptr(), *h.stride()[:2],
-            hn.data_ptr(), _p(states), T, B, D, _p(ws))
-    return h, hn, states
-
-
-def _scan_backward(ctx, dh, dhn):
-    if dh is None and dhn is None:
-        return None, None, None, None, None
-    x, gate, reset, lengths, states = ctx.saved_tensors
-    T, B, D = x.shape
-    dtype, device = x.dtype, x.device
-    if dh is None:
-        dh = torch.zeros(D, dtype=dtype, device=device).expand(T, B, D)
-    elif dh.dtype != dtype or (dh.stride(-1) != 1 and D != 1):
-        dh = dh.to(dtype).contiguous()
-    if dhn is not None and not (dhn.dtype == torch.float32 and dhn.is_contiguous()):
-        dhn = dhn.to(torch.float32).contiguous()
-    dx, dgate = _like_rows(x), _like_rows(x)
-    dh0 = torch.empty((B, D), dtype=torch.float32, device=device) if ctx.needs_input_grad[2] else None
-    ws = _bytes(ctx.ws_bytes, device)
-    strides = dx.stride()[:2]
-    _launch(device.index, lib.rlpyt_gated_scan_bwd, _DTYPES[dtype], x.data_ptr(), *x.stride()[:2],
-            gate.data_ptr(), *gate.stride()[:2], dh.data_ptr(), *dh.stride()[:2], _p(dhn), _p(reset), _p(lengths),
-            states.data_ptr(), dx.data_ptr(), *strides, dgate.data_ptr(), *strides, _p(dh0), T, B, D, _p(ws))
-    if dh0 is not None and ctx.h0_dtype != torch.float32:
-        dh0 = dh0.to(ctx.h0_dtype)
-    return dx, dgate, dh0, None, None
-
-
-class _GatedScan(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gate, h0, reset, lengths):
-        h0_dtype = None if h0 is None else h0.dtype
-        h, hn, states = _scan_forward(x, gate, _state32(h0), reset, lengths, True)
-        ctx.save_for_backward(x, gate, reset, lengths, states)
-        ctx.h0_dtype = h0_dtype
-        ctx.ws_bytes = lib.rlpyt_gated_scan_workspace_bytes(*x.shape)
-        ctx.set_materialize_grads(False)
-        return h, hn
-
-    backward = _backward(_scan_backward)
-
-
-def _state32(h0):
-    if h0 is None or (h0.dtype == torch.float32 and h0.is_contiguous()):
-        return h0
-    return h0.detach().to(torch.float32).contiguous()
-
-
 def _reset_bytes(reset):
     return (reset if reset.dtype in _BYTES else reset != 0).contiguous()
 
@@ -190,9 +96,7 @@ def gated_scan(x, gate, h0=None, reset=None, lengths=None):
             x = x.contiguous()
         if gate.stride(-1) != 1:
             gate = gate.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (h0 is not None and h0.requires_grad)):
-        return _GatedScan.apply(x, gate, h0, reset, lengths)
-    return _scan_forward(x, gate, _state32(h0), reset, lengths, False)[:2]
+    return _seqops.gated_scan(x, gate, h0, reset, lengths)
 
 
 def gated_scan_step(x, gate, state, reset=None):
@@ -214,17 +118,12 @@ def gated_scan_step(x, gate, state, reset=None):
     _need_device("gated_scan_step", x, gate, state, reset)
     if reset is not None and not (reset.dtype in _BYTES and reset.is_contiguous()):
         reset = _reset_bytes(reset)
-    B, D = shape
-    if D != 1:
+    if shape[1] != 1:
         if x.stride(-1) != 1:
             x = x.contiguous()
         if gate.stride(-1) != 1:
             gate = gate.contiguous()
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    _launch(x.get_device(), lib.rlpyt_gated_scan_step, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), gate.data_ptr(),
-            gate.stride(0), _p(reset), state.data_ptr(), y.data_ptr(), B, D)
-    torch.autograd.graph.increment_version(state)   # written through a raw pointer
-    return y
+    return _seqops.gated_scan_step(x, gate, state, reset)
 
 
 # --------------------------------------------------------------------------------------
@@ -256,43 +155,8 @@ def _numbers(t):
     return t.detach().to(torch.float32).contiguous()
 
 
-def _loss_forward(rows, numbers, coeffs, want_grad):
-    """One pass over ``rows [N, V]`` -> loss, scalars [5], gradient [N, V] or None."""
-    N, V = rows.shape
-    code, device = _DTYPES[rows.dtype], rows.device
-    scalars = torch.empty(5, dtype=torch.float32, device=device)
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    grad = torch.empty((N, V), dtype=rows.dtype, device=device) if want_grad else None
-    ws = _bytes(lib.rlpyt_policy_loss_workspace_bytes(code, N, V), device)
-    _launch(device.index, lib.rlpyt_policy_kl_loss_fwd_bwd, code, rows.data_ptr(), rows.stride(0),
-            *(_p(t) for t in numbers), N, V, *coeffs, loss.data_ptr(), scalars.data_ptr(), _p(grad), ws.data_ptr())
-    return loss, scalars, grad
-
-
-def _loss_backward(ctx, g_loss, _g_scalars):
-    grad, ctx.grad = ctx.grad, None
-    if grad is None:
-        raise RuntimeError("policy_kl_loss: its gradient went out with the first backward pass (it is scaled in place); "
-                           "run the loss again")
-    if not _is_unit_seed(g_loss):
-        _launch(grad.get_device(), lib.rlpyt_scale_unless_one, _DTYPES[grad.dtype], grad.data_ptr(), grad.numel(),
-                g_loss.data_ptr())
-    return (grad if ctx.shape is None else grad.reshape(ctx.shape)), None, None, None
-
-
-class _PolicyKlLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, rows, numbers, coeffs):
-        loss, scalars, grad = _loss_forward(rows, numbers, coeffs, True)
-        ctx.grad, ctx.shape = grad, None if logits.dim() == 2 else logits.shape
-        ctx.mark_non_differentiable(scalars)
-        return loss, scalars
-
-    backward = _backward(_loss_backward)
-
-
 def policy_kl_loss(logits, action, old_logp, advantage, ref_logp=None, valid=None, clip_low=0.2, clip_high=0.2,
-                   kl_coeff=0., entropy_coeff=0.):
+                   kl_coeff=0., entropy_coeff=0., grad_scale=1.):
     """Clipped policy loss with a KL term and an entropy bonus over ``softmax(logits)``, as one fused forward
     and backward pass over the logits::
 
@@ -306,6 +170,10 @@ def policy_kl_loss(logits, action, old_logp, advantage, ref_logp=None, valid=Non
     Returns ``(loss, scalars)``: ``loss`` is differentiable w.r.t. ``logits`` (one backward pass a call: the
     gradient comes out of the forward pass, is scaled in place and handed on), ``scalars = [loss, pi_loss, kl,
     entropy, clipped share]`` (detached).
+
+    The gradient is rounded to the type of ``logits`` in the forward pass, for an incoming gradient of ``grad_scale``;
+    another one costs a pass over it, and a second rounding where their ratio is no power of two.  A loss that is scaled
+    against float16's underflow (``(S * loss).backward()``) needs ``grad_scale=S``.
 
     Logits of -inf are actions that are not allowed.  Rows whose ``valid`` is 0 are not read and have a zero
     gradient, also where their action is out of range; nothing valid gives a loss of 0.  A row that allows
@@ -321,13 +189,14 @@ def policy_kl_loss(logits, action, old_logp, advantage, ref_logp=None, valid=Non
         _refuse("policy_kl_loss: 0 <= clip_low <= 1 and 0 <= clip_high are needed")
     if ref_logp is None and kl_coeff != 0.:
         _refuse("policy_kl_loss: kl_coeff needs ref_logp")
+    if not 0. < grad_scale < float("inf"):
+        _refuse("policy_kl_loss: a positive grad_scale is needed")
     rows, action = _logit_rows("policy_kl_loss", logits, action)
     _need_device("policy_kl_loss", rows, old_logp, advantage, ref_logp, valid)
-    numbers = (action, _numbers(old_logp), _numbers(advantage), _numbers(ref_logp), _numbers(valid))
-    coeffs = (float(clip_low), float(clip_high), float(kl_coeff), float(entropy_coeff))
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _PolicyKlLoss.apply(logits, rows, numbers, coeffs)
-    return _loss_forward(rows, numbers, coeffs, False)[:2]
+    seed = _unit_seeds.get(logits.device)
+    return _seqops.policy_kl_loss(logits, rows, action, _numbers(old_logp), _numbers(advantage), _numbers(ref_logp),
+                                  _numbers(valid), clip_low, clip_high, kl_coeff, entropy_coeff, grad_scale,
+                                  0 if seed is None else seed.data_ptr())
 
 
 def action_logp(logits, action):
@@ -335,15 +204,7 @@ def action_logp(logits, action):
     bfloat16 or float16): what ``policy_kl_loss`` takes as ``old_logp`` and ``ref_logp``.  Reads the logits once; not
     differentiable.  A row of -inf only gives ``(-inf, 0)``, an action outside 0 .. V-1 NaN."""
     rows, action = _logit_rows("action_logp", logits, action)
-    N, V = rows.shape
-    code, device = _DTYPES[rows.dtype], rows.device
-    lead = logits.shape[:-1]
-    logp = torch.empty(lead, dtype=torch.float32, device=device)
-    entropy = torch.empty(lead, dtype=torch.float32, device=device)
-    ws = _bytes(lib.rlpyt_policy_loss_workspace_bytes(code, N, V), device)
-    _launch(device.index, lib.rlpyt_action_logp, code, rows.data_ptr(), rows.stride(0), action.data_ptr(), N, V,
-            logp.data_ptr(), entropy.data_ptr(), ws.data_ptr())
-    return logp, entropy
+    return _seqops.action_logp(logits, rows, action)
 
 
 # --------------------------------------------------------------------------------------
@@ -399,10 +260,12 @@ def orthogonalize(mats, steps=5, coeffs=NS_COEFFS, eps=1e-7):
         ins, lds, dsts, rows, cols = zip(*table)
         ins, dsts = (ctypes.c_void_p * k)(*ins), (ctypes.c_void_p * k)(*dsts)
         lds, rows, cols = ((ctypes.c_int64 * k)(*v) for v in (lds, rows, cols))
-        ws = _bytes(lib.rlpyt_orthogonalize_workspace_bytes(rows, cols, k), device)
-        _launch(device.index, lib.rlpyt_orthogonalize, _DTYPES[dtype], ins, lds, dsts, rows, cols, k, int(steps),
-                *map(float, coeffs), float(eps), _p(ws))
+        ws = torch.empty(lib.rlpyt_orthogonalize_workspace_bytes(rows, cols, k), dtype=torch.uint8, device=device)
+        with torch.cuda.device(device):
+            check(lib.rlpyt_orthogonalize(_DTYPES[dtype], ins, lds, dsts, rows, cols, k, int(steps), *map(float, coeffs),
+                                          float(eps), ws.data_ptr(), torch.cuda.current_stream().cuda_stream),
+                  "rlpyt_orthogonalize")
     return outs[0] if single else outs
 
 
-from .ops import _is_unit_seed  # noqa: E402  (ops imports this module at its end)
+from .ops import _unit_seeds  # noqa: E402  (ops imports this module at its end)

@@ -225,7 +225,7 @@ class Muon(torch.optim.Optimizer):
     not Adam's 1e-3.
 
     An algorithm takes it as ``OptimCls=Muon``; ``clip_and_step`` is what the algorithms here call.  All matrices of a step go
-    through the same few launches; float32, bfloat16 and float16 parameters on the device."""
+    through the same few launches.  Parameters of any floating type on the device; buffers and updates are float32."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0., ns_steps=5,
                  ns_coeffs=(3.4445, -4.7750, 2.0315), ns_eps=1e-7, adam_lr_ratio=0.05, adam_betas=(0.9, 0.999),
@@ -248,15 +248,24 @@ class Muon(torch.optim.Optimizer):
             self._vector_step(group, [p for p in params if p.dim() < 2])
         return loss
 
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # (torch has cast the buffers to their parameters' types)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
+            for k, v in state_dict["state"].get(i, {}).items():
+                if isinstance(v, torch.Tensor) and v.is_floating_point():
+                    self.state[p][k] = v.detach().to(p.device, torch.float32, copy=True)
+
     def _matrix_step(self, group, params):
         if not params:
             return
         from .ops import orthogonalize
         beta, lr = group["momentum"], float(group["lr"])
-        grads = [p.grad for p in params]
+        grads = [p.grad.float() for p in params]
         for p in params:
             if not self.state[p]:
-                self.state[p]["momentum_buffer"] = torch.zeros_like(p)
+                self.state[p]["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
         bufs = [self.state[p]["momentum_buffer"] for p in params]
         torch._foreach_lerp_(bufs, grads, 1. - beta)
         updates = torch._foreach_lerp(grads, bufs, beta) if group["nesterov"] else bufs
@@ -273,10 +282,11 @@ class Muon(torch.optim.Optimizer):
             return
         b1, b2 = group["adam_betas"]
         lr = float(group["lr"]) * group["adam_lr_ratio"]
-        grads = [p.grad for p in params]
+        grads = [p.grad.float() for p in params]
         for p in params:
             if not self.state[p]:
-                self.state[p].update(step=0, exp_avg=torch.zeros_like(p), exp_avg_sq=torch.zeros_like(p))
+                self.state[p].update(step=0, exp_avg=torch.zeros_like(p, dtype=torch.float32),
+                                     exp_avg_sq=torch.zeros_like(p, dtype=torch.float32))
             self.state[p]["step"] += 1
         avgs, squares = ([self.state[p][k] for p in params] for k in ("exp_avg", "exp_avg_sq"))
         torch._foreach_lerp_(avgs, grads, 1. - b1)
@@ -287,7 +297,7 @@ class Muon(torch.optim.Optimizer):
         for p, m, v in zip(params, avgs, squares):
             n = self.state[p]["step"]
             denom = (v / (1. - b2 ** n)).sqrt_().add_(group["adam_eps"])
-            p.addcdiv_(m, denom, value=-lr / (1. - b1 ** n))
+            p.add_(m / denom, alpha=-lr / (1. - b1 ** n))
 
     @torch.no_grad()
     def clip_and_step(self, max_norm, norm_out=None):

@@ -37,6 +37,8 @@ z = torch.zeros
     lambda: ops.policy_kl_loss(z(3, 4), z(3).long(), z(3), z(3), clip_low=1.5),
     lambda: ops.policy_kl_loss(z(3, 4), z(3).long(), z(3), z(3), clip_high=-0.1),
     lambda: ops.policy_kl_loss(z(3, 4), z(3).long(), z(3), z(3), clip_high=float("nan")),
+    lambda: ops.policy_kl_loss(z(3, 4), z(3).long(), z(3), z(3), grad_scale=0.),
+    lambda: ops.policy_kl_loss(z(3, 4), z(3).long(), z(3), z(3), grad_scale=float("inf")),
     lambda: ops.action_logp(z(3, 4), z(3)),
     lambda: ops.action_logp(z(3, 4).long(), z(3).long()),
     lambda: ops.orthogonalize(z(4)),
@@ -92,14 +94,14 @@ def test_entry_points_validate_without_a_gpu():
     assert lib.rlpyt_gated_scan_step(0, None, 0, None, 0, None, None, None, 0, 4, None) == 0
     assert lib.rlpyt_gated_scan_step(0, None, 0, None, 0, None, None, None, 2, 4, None) != 0
     loss = lib.rlpyt_policy_kl_loss_fwd_bwd
-    assert loss(0, p, 4, p, p, p, None, None, 2, 0, .2, .2, 0., 0., p, p, None, p, None) != 0
-    assert loss(0, None, 4, p, p, p, None, None, 2, 4, .2, .2, 0., 0., p, p, None, p, None) != 0
-    assert loss(0, p, 4, p, p, p, None, None, 2, 4, .2, .2, 0., 0., None, p, None, p, None) != 0
-    assert loss(0, p, 4, p, p, p, None, None, 2, 4, .2, .2, 0., 0., p, p, None, None, None) != 0
+    assert loss(0, p, 4, p, p, p, None, None, 2, 0, .2, .2, 0., 0., 1., p, p, None, p, None) != 0
+    assert loss(0, None, 4, p, p, p, None, None, 2, 4, .2, .2, 0., 0., 1., p, p, None, p, None) != 0
+    assert loss(0, p, 4, p, p, p, None, None, 2, 4, .2, .2, 0., 0., 1., None, p, None, p, None) != 0
+    assert loss(0, p, 4, p, p, p, None, None, 2, 4, .2, .2, 0., 0., 1., p, p, None, None, None) != 0
     assert lib.rlpyt_action_logp(0, None, 4, None, 0, 4, None, None, None, None) == 0
     assert lib.rlpyt_action_logp(0, None, 4, None, 2, 4, None, None, None, None) != 0
-    assert lib.rlpyt_scale_unless_one(0, None, 0, None, None) == 0
-    assert lib.rlpyt_scale_unless_one(0, None, 4, None, None) != 0
+    assert lib.rlpyt_scale_unless_one(0, None, 0, None, 1., None) == 0
+    assert lib.rlpyt_scale_unless_one(0, None, 4, None, 1., None) != 0
     one = (ctypes.c_void_p * 1)(p.value)
     side, big = (ctypes.c_int64 * 1)(4), (ctypes.c_int64 * 1)(1 << 20)
     orth = lib.rlpyt_orthogonalize

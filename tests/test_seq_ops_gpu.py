@@ -341,10 +341,12 @@ def run_loss(logits, action, old, adv, ref, w, **kw):
     return loss.detach(), scalars, logits.grad
 
 
-def loss_close(loss, scalars, grad, want_s, want_g):
-    # a row: |x - max| < 64 in e^(x - max) and 2^-20 for the sum, of terms of the size of the row's largest
+def loss_close(loss, scalars, grad, want_s, want_g, cancel=0.):
+    # a row: |x - max| < 64 in e^(x - max) and 2^-20 for the sum, of terms of the size of the row's largest.  cancel: what
+    # the entropy's part c_H p (log p + H) w / sum w consists of: log p and H are each known to err relative, and in a row that
+    # is all but uniform and has no other part (a clipped ratio, a tiny advantage) they cancel, the row's largest with them
     err = (64 + 4) * 2. ** -24 + 2. ** -20
-    top = want_g.abs().amax(-1, keepdim=True)
+    top = want_g.abs().amax(-1, keepdim=True) + cancel
     assert bool(((grad.double() - want_g).abs() <=
                  HALF[grad.dtype] * want_g.abs() + 4 * err * top + torch.finfo(grad.dtype).tiny).all()), \
         float(((grad.double() - want_g).abs() - HALF[grad.dtype] * want_g.abs()).max())
@@ -499,6 +501,13 @@ def test_policy_kl_loss_backward_scale_and_second_pass():
     one = ops.unit_seed(logits.device)
     torch.autograd.backward(call(), one)
     assert torch.equal(logits.grad, grad)
+    logits.grad = None
+    loss = ops.policy_kl_loss(logits, *data[1:4], ref_logp=data[4], valid=data[5], grad_scale=1024., **KW)[0]
+    (1024. * loss).backward()
+    assert torch.equal(logits.grad, grad * 1024.)
+    logits.grad = None
+    ops.policy_kl_loss(logits, *data[1:4], ref_logp=data[4], valid=data[5], grad_scale=1024., **KW)[0].backward()
+    assert torch.equal(logits.grad, grad)
     loss = call()
     loss.backward(retain_graph=True)
     with pytest.raises(RuntimeError, match="first backward"):
@@ -509,6 +518,53 @@ def test_policy_kl_loss_backward_scale_and_second_pass():
     loss, scalars = ops.policy_kl_loss(empty, none.long(), none, none)
     loss.backward()
     assert float(loss.detach()) == 0. and empty.grad.shape == (0, 5)
+
+
+def test_policy_kl_loss_float16_gradients_that_underflow_unscaled():
+    N, V, S = 2000, 3000, 65536.
+    logits, action, old, adv, ref, _ = loss_data(N, V, torch.float16, 71)
+    leaf = logits.clone().requires_grad_(True)
+    loss, _ = ops.policy_kl_loss(leaf, action, old, adv, ref_logp=ref, grad_scale=S, **KW)
+    (loss * S).backward()
+    _, want = loss64(logits, action, old, adv, ref, None, 0.2, 0.3)
+    want = want * S
+    err = (64 + 4) * 2. ** -24 + 2. ** -20          # as in loss_close, beside float16's subnormals: steps of 2^-24
+    assert bool(((leaf.grad.double() - want).abs() <= HALF[torch.float16] * want.abs() + 2. ** -25
+                 + 4 * err * want.abs().amax(-1, keepdim=True)).all())
+    assert bool((leaf.grad != 0)[want.abs() > 2. ** -24].all())          # nothing that float16 holds is lost
+
+
+def test_policy_kl_loss_many_rows_go_in_slices():
+    N, V = (1 << 21) + 70, 3
+    g = gen(72)
+    logits = torch.randn(N, V, device=DEV, generator=g)
+    action = torch.randint(0, V, (N,), device=DEV, generator=g)
+    old = torch.log_softmax(logits, -1).gather(-1, action[:, None]).squeeze(-1) - 0.05
+    adv = torch.randn(N, device=DEV, generator=g)
+    out = run_loss(logits, action, old, adv, None, None, entropy_coeff=0.02, **KW)
+    want = loss64(logits, action, old, adv, None, None, 0.2, 0.3, 0., 0.02)
+    loss_close(*out, *want, cancel=0.02 * math.log(3) / N)
+
+
+def test_policy_kl_loss_of_one_row_without_leading_axes():
+    logits = torch.randn(50, device=DEV, generator=gen(73), requires_grad=True)
+    action = torch.tensor(7, device=DEV)
+    old, ent = ops.action_logp(logits.detach(), action)
+    assert old.shape == () and ent.shape == ()
+    loss, _ = ops.policy_kl_loss(logits, action, old, torch.tensor(2., device=DEV))
+    loss.backward()
+    assert logits.grad.shape == (50,) and abs(float(loss.detach()) + 2.) < 1e-5
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(5, 2, 4, device=DEV, requires_grad=True)
+    gate = torch.randn(5, 2, 4, device=DEV)
+    h, _ = ops.gated_scan(x, gate)
+    g, = torch.autograd.grad(h.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    want, = torch.autograd.grad(ops.gated_scan(x, gate)[0].sum(), x)
+    assert torch.equal(g.detach(), want)
 
 
 def test_policy_kl_loss_offsets_past_32_bits():
@@ -578,7 +634,7 @@ def test_orthogonalize_of_lists_batches_and_views():
             orth_close(oi, orth64(gi))
     assert torch.equal(outs[0], outs[-1])
     alone = ops.orthogonalize(mats[1])
-    assert torch.equal(alone, outs[1])       # a matrix' result does not depend on its company
+    assert torch.equal(alone, outs[1])       # (these few are too small to be split differently in company)
 
 
 def test_orthogonalize_options_and_edges():
@@ -724,6 +780,28 @@ def test_muon_steps(nesterov, decay):
     opt.clip_and_step(1.)
     opt2.clip_and_step(1.)
     assert all(torch.equal(p, o) for p, o in zip(params, other))
+
+
+def test_muon_of_16_bit_parameters_keeps_its_buffers_in_32():
+    from rlpyt_amd.optim import Muon
+    mk = gen(131)
+    w = torch.nn.Parameter(torch.randn(60, 90, device=DEV, generator=mk).bfloat16())
+    v = torch.nn.Parameter(torch.zeros(9, device=DEV, dtype=torch.bfloat16))
+    start = w.detach().clone()
+    opt = Muon([w, v], lr=0.5)
+    grads = [torch.randn(60, 90, device=DEV, generator=mk).bfloat16() for _ in range(2)]
+    for g in grads:
+        w.grad, v.grad = g.clone(), torch.ones_like(v)
+        opt.step()
+    assert opt.state[w]["momentum_buffer"].dtype == torch.float32 == opt.state[v]["exp_avg"].dtype
+    want = muon64(start, grads, 0.5, 0.95, True, 0.)
+    # two roundings of the weights, beside the updates' own error
+    err = 2 * HALF[torch.bfloat16] * float(want.norm()) + 2 * 0.5 * 4 * 484 * 2. ** -23
+    assert float((w.detach().double() - want).norm()) <= err
+    other = Muon([torch.nn.Parameter(w.detach().clone()), torch.nn.Parameter(v.detach().clone())])
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))
+    buf = other.state[other.param_groups[0]["params"][0]]["momentum_buffer"]
+    assert buf.dtype == torch.float32 and torch.equal(buf, opt.state[w]["momentum_buffer"])
 
 
 def test_a_recurrent_policy_trains_with_the_operators_together():
