@@ -65,6 +65,16 @@ __host__ __device__ static inline int64_t ceil_div(int64_t a, int64_t b) { retur
 
 constexpr int kWave = 64;  // CDNA wavefront width
 
+// Element types of a kernel's tensors, by names that read the same in its mangled name and in the variant registry.
+struct Bf16 {};
+struct Half {};
+template <typename ET>
+struct Elem { typedef ET type; };
+template <>
+struct Elem<Bf16> { typedef __bf16 type; };
+template <>
+struct Elem<Half> { typedef _Float16 type; };
+
 // Wave-level sum over the 64 lanes (butterfly; every lane gets the total).
 template <typename T>
 __device__ __forceinline__ T wave_sum(T v) {

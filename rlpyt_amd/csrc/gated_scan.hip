@@ -178,8 +178,9 @@ __device__ __forceinline__ void segment_carry(const Args& p, const Lane& l, int 
 }
 
 // Forward.  AGG: reduce the segment to its map, write nothing else.
-template <typename E, int V, bool RESET, bool LEN, bool AGG>
+template <typename ET, int V, bool RESET, bool LEN, bool AGG>
 __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_fwd_kernel(const Args p) {
+  typedef typename Elem<ET>::type E;
   typedef typename Vec<E, V>::type VE;
   __shared__ float2 lds[2][kMaxWaves][kWave * V];
   const Lane l = lane_of<V, LEN>(p);
@@ -303,8 +304,9 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_fwd_kernel(const Ar
 
 // Backward, from the last window to the first.  The map of a step acts on R_t = (1 - z_{t+1}) k_{t+1}
 // G_{t+1}, what comes from behind: R_{t-1} = a_t k_t (dh_t + R_t).
-template <typename E, int V, bool RESET, bool LEN, bool AGG>
+template <typename ET, int V, bool RESET, bool LEN, bool AGG>
 __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(const Args p) {
+  typedef typename Elem<ET>::type E;
   typedef typename Vec<E, V>::type VE;
   __shared__ float2 lds[2][kMaxWaves][kWave * V];
   __shared__ float ldh[2][AGG ? 1 : kMaxWaves][kWave * V];   // the maps' H, forward
@@ -484,10 +486,13 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(const Ar
 }
 
 // One step: read x, gate and the state, write the state and the output; one lane per V channels.
-template <typename E, int V>
+template <typename ET, int V>
 __global__ __launch_bounds__(256) void gated_scan_step_kernel(
-    const E* __restrict__ x, int64_t xbs, const E* __restrict__ gate, int64_t gbs,
-    const uint8_t* __restrict__ reset, float* __restrict__ state, E* __restrict__ y, int64_t C, int D) {
+    const void* __restrict__ xp, int64_t xbs, const void* __restrict__ gp, int64_t gbs,
+    const uint8_t* __restrict__ reset, float* __restrict__ state, void* __restrict__ yp, int64_t C, int D) {
+  typedef typename Elem<ET>::type E;
+  const E *x = (const E*)xp, *gate = (const E*)gp;
+  E* y = (E*)yp;
   typedef typename Vec<E, V>::type VE;
   typedef typename Vec<float, V>::type VF;
   const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
@@ -542,38 +547,39 @@ bool fits(const void* ptr, Stream st, int D, int V, int size) {
   return ((uintptr_t)ptr & (V * size - 1)) == 0 && st.ts % V == 0 && st.bs % V == 0 && D % V == 0;
 }
 
-template <bool FWD, typename E, int V, bool RESET, bool LEN>
+template <bool FWD, typename ET, int V, bool RESET, bool LEN>
 int launch(const Args& p, const Plan& q, int64_t tiles, hipStream_t s) {
   const dim3 block(64 * q.W), grid((unsigned)tiles, (unsigned)q.S);
   if (FWD) {
-    if (q.S > 1) RL_LAUNCH((gated_scan_fwd_kernel<E, V, RESET, LEN, true>), grid, block, 0, s, p);
-    RL_LAUNCH((gated_scan_fwd_kernel<E, V, RESET, LEN, false>), grid, block, 0, s, p);
+    if (q.S > 1) RL_LAUNCH((gated_scan_fwd_kernel<ET, V, RESET, LEN, true>), grid, block, 0, s, p);
+    RL_LAUNCH((gated_scan_fwd_kernel<ET, V, RESET, LEN, false>), grid, block, 0, s, p);
   } else {
-    if (q.S > 1) RL_LAUNCH((gated_scan_bwd_kernel<E, V, RESET, LEN, true>), grid, block, 0, s, p);
-    RL_LAUNCH((gated_scan_bwd_kernel<E, V, RESET, LEN, false>), grid, block, 0, s, p);
+    if (q.S > 1) RL_LAUNCH((gated_scan_bwd_kernel<ET, V, RESET, LEN, true>), grid, block, 0, s, p);
+    RL_LAUNCH((gated_scan_bwd_kernel<ET, V, RESET, LEN, false>), grid, block, 0, s, p);
   }
   RL_LAUNCH_CHECK();
   return RLPYT_OK;
 }
 
-template <bool FWD, typename E, int V>
+template <bool FWD, typename ET, int V>
 int dispatch(const Args& p, hipStream_t s) {
   const int64_t tiles = tiles_of(p.B, p.D, V);
   const Plan q = plan_of(p.T, tiles);
   Args a = p;
   a.seg = q.seg;
-  if (p.reset && p.lengths) return launch<FWD, E, V, true, true>(a, q, tiles, s);
-  if (p.reset) return launch<FWD, E, V, true, false>(a, q, tiles, s);
-  if (p.lengths) return launch<FWD, E, V, false, true>(a, q, tiles, s);
-  return launch<FWD, E, V, false, false>(a, q, tiles, s);
+  if (p.reset && p.lengths) return launch<FWD, ET, V, true, true>(a, q, tiles, s);
+  if (p.reset) return launch<FWD, ET, V, true, false>(a, q, tiles, s);
+  if (p.lengths) return launch<FWD, ET, V, false, true>(a, q, tiles, s);
+  return launch<FWD, ET, V, false, false>(a, q, tiles, s);
 }
 
-template <bool FWD, typename E>
+template <bool FWD, typename ET>
 int pick(const Args& p, hipStream_t s) {
+  typedef typename Elem<ET>::type E;
   if constexpr (sizeof(E) == 2) {
-    if (channels(2, p.D) == 2) return dispatch<FWD, E, 2>(p, s);
+    if (channels(2, p.D) == 2) return dispatch<FWD, ET, 2>(p, s);
   }
-  return dispatch<FWD, E, 1>(p, s);
+  return dispatch<FWD, ET, 1>(p, s);
 }
 
 bool sizes_ok(int64_t T, int64_t B, int64_t D) {
@@ -616,8 +622,8 @@ extern "C" int rlpyt_gated_scan_fwd(int dtype, const void* x, int64_t x_ts, int6
   p.T = (int)T, p.B = (int)B, p.D = (int)D;
   hipStream_t s = (hipStream_t)stream;
   if (dtype == F32) return pick<true, float>(p, s);
-  if (dtype == BF16) return pick<true, __bf16>(p, s);
-  return pick<true, _Float16>(p, s);
+  if (dtype == BF16) return pick<true, Bf16>(p, s);
+  return pick<true, Half>(p, s);
 }
 
 extern "C" int rlpyt_gated_scan_bwd(int dtype, const void* x, int64_t x_ts, int64_t x_bs, const void* gate,
@@ -641,25 +647,26 @@ extern "C" int rlpyt_gated_scan_bwd(int dtype, const void* x, int64_t x_ts, int6
   p.T = (int)T, p.B = (int)B, p.D = (int)D;
   hipStream_t s = (hipStream_t)stream;
   if (dtype == F32) return pick<false, float>(p, s);
-  if (dtype == BF16) return pick<false, __bf16>(p, s);
-  return pick<false, _Float16>(p, s);
+  if (dtype == BF16) return pick<false, Bf16>(p, s);
+  return pick<false, Half>(p, s);
 }
 
 namespace {
-template <typename E>
+template <typename ET>
 int step_of(const void* x, int64_t xbs, const void* gate, int64_t gbs, const uint8_t* reset, float* state,
             void* y, int64_t B, int64_t D, hipStream_t s) {
+  typedef typename Elem<ET>::type E;
   const Stream xs = {0, xbs}, gs = {0, gbs}, dense = {0, D};
   const int64_t C = B * D;
   const int size = (int)sizeof(E);
   const bool wide = fits(x, xs, (int)D, 2, size) && fits(gate, gs, (int)D, 2, size) && fits(y, dense, (int)D, 2, size) &&
                     fits(state, dense, (int)D, 2, 4);
   if (wide)
-    RL_LAUNCH((gated_scan_step_kernel<E, 2>), dim3((unsigned)ceil_div(C, 512)), dim3(256), 0, s, (const E*)x, xbs,
-              (const E*)gate, gbs, reset, state, (E*)y, C, (int)D);
+    RL_LAUNCH((gated_scan_step_kernel<ET, 2>), dim3((unsigned)ceil_div(C, 512)), dim3(256), 0, s, x, xbs,
+              gate, gbs, reset, state, y, C, (int)D);
   else
-    RL_LAUNCH((gated_scan_step_kernel<E, 1>), dim3((unsigned)ceil_div(C, 256)), dim3(256), 0, s, (const E*)x, xbs,
-              (const E*)gate, gbs, reset, state, (E*)y, C, (int)D);
+    RL_LAUNCH((gated_scan_step_kernel<ET, 1>), dim3((unsigned)ceil_div(C, 256)), dim3(256), 0, s, x, xbs,
+              gate, gbs, reset, state, y, C, (int)D);
   RL_LAUNCH_CHECK();
   return RLPYT_OK;
 }
@@ -674,6 +681,6 @@ extern "C" int rlpyt_gated_scan_step(int dtype, const void* x, int64_t x_bs, con
   RL_CHECK_ARG(x && gate && state && y, RLPYT_EINVAL, "rlpyt_gated_scan_step: null pointer");
   hipStream_t s = (hipStream_t)stream;
   if (dtype == F32) return step_of<float>(x, x_bs, gate, g_bs, reset, state, y, B, D, s);
-  if (dtype == BF16) return step_of<__bf16>(x, x_bs, gate, g_bs, reset, state, y, B, D, s);
-  return step_of<_Float16>(x, x_bs, gate, g_bs, reset, state, y, B, D, s);
+  if (dtype == BF16) return step_of<Bf16>(x, x_bs, gate, g_bs, reset, state, y, B, D, s);
+  return step_of<Half>(x, x_bs, gate, g_bs, reset, state, y, B, D, s);
 }

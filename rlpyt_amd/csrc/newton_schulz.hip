@@ -58,8 +58,9 @@ __device__ __forceinline__ int find(const Mats* __restrict__ t, int kind, int ti
   return __builtin_amdgcn_readfirstlane(__popcll(__ballot(behind)) - 1);
 }
 
-template <typename E>
+template <typename ET>
 __global__ __launch_bounds__(256) void ns_norm_kernel(const Mats t, Mats* __restrict__ table) {
+  typedef typename Elem<ET>::type E;
   constexpr int n16 = 16 / sizeof(E);
   typedef E vec __attribute__((ext_vector_type(n16)));
   __shared__ double scratch[16];
@@ -110,17 +111,18 @@ __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
 }
 
 // X_0 and its transpose from 32 x 32 tiles of the input
-template <typename E>
+template <typename ET>
 __global__ __launch_bounds__(256) void ns_load_kernel(const Mats* __restrict__ t, double eps) {
+  typedef typename Elem<ET>::type E;
   __shared__ float tile[32][33];
-  __shared__ float factor;
+  __shared__ double factor;
   const int i = find(t, LOAD, blockIdx.x);
   const Mat M = t->m[i];
   if (threadIdx.x < kWave) {
     double s = 0.0;
     for (int k = threadIdx.x; k < kNormBlocks; k += kWave) s += M.norm[k];
     s = wave_sum(s);
-    if (threadIdx.x == 0) factor = (float)((double)kScale / (sqrt(s) + eps));
+    if (threadIdx.x == 0) factor = s > 0.0 ? (double)kScale / (sqrt(s) + eps) : s;   // (a NaN stays one)
   }
   __syncthreads();
   const int block = blockIdx.x - t->first[LOAD][i], tn = M.np / 32;
@@ -129,7 +131,7 @@ __global__ __launch_bounds__(256) void ns_load_kernel(const Mats* __restrict__ t
   for (int k = ly; k < 32; k += 8) {   // coalesced along the input's rows
     const int r = M.tall ? c0 + k : r0 + k, c = M.tall ? r0 + lx : c0 + lx;
     float v = 0.f;
-    if (r < M.rows && c < M.cols) v = (float)((const E*)M.in)[(int64_t)r * M.ld + c] * factor;
+    if (r < M.rows && c < M.cols) v = (float)((double)(float)((const E*)M.in)[(int64_t)r * M.ld + c] * factor);
     if (M.tall) tile[lx][k] = v;
     else tile[k][lx] = v;
   }
@@ -311,9 +313,10 @@ __device__ __forceinline__ int place(int row, int k) { return k ^ ((row >> 1) & 
 // the even and of the odd ones, which are 128 bytes apart.  (Permuted by row & 7: half of all reads took 4 cycles more.)
 // Tiles from `full` on are split along K into S slices of a workgroup each, whose sums go to `part` for ns_finish_kernel: the
 // tiles that would make a round of their own on an idle chip.
-template <int MODE, int T, int G_, int NS, typename E>
+template <int MODE, int T, int G_, int NS, typename ET>
 __global__ __launch_bounds__((Shape<T, G_>::threads)) void ns_product_kernel(const Mats* __restrict__ t, int cur, Coeffs f,
                                                                           int full, int S, float* __restrict__ part) {
+  typedef typename Elem<ET>::type E;
   typedef Shape<T, G_> G;
   constexpr int NX = G::nx, NY = G::ny, L = 2 * G::passes, KG = G::sets;
   __shared__ __attribute__((aligned(16))) uint8_t lds[NS][KG][2][T * 128];
@@ -448,9 +451,10 @@ __global__ __launch_bounds__((Shape<T, G_>::threads)) void ns_product_kernel(con
 }
 
 // Adds the slices of the split tiles, in order: a wave per 32 x 32 block of T = 256 and 128,
-template <int MODE, int T, typename E>
+template <int MODE, int T, typename ET>
 __global__ __launch_bounds__(64) void ns_finish_kernel(const Mats* __restrict__ t, int cur, Coeffs f, int full, int S,
                                                        const float* __restrict__ part) {
+  typedef typename Elem<ET>::type E;
   constexpr int N = T / 32;
   const int tile = blockIdx.x / (N * N), block = blockIdx.x % (N * N);
   const Where w = where<MODE, T>(t, full + tile);
@@ -465,13 +469,12 @@ __global__ __launch_bounds__(64) void ns_finish_kernel(const Mats* __restrict__ 
 }
 
 // and 16 rows of a 64 x 64 tile by a workgroup of two waves.
-template <int MODE, typename E>
-__global__ __launch_bounds__(128) void ns_finish64_kernel(const Mats* __restrict__ t, int cur, Coeffs f, int full, int S,
+__global__ __launch_bounds__(128) void ns_finish64_kernel(const Mats* __restrict__ t, int full, int S,
                                                           const float* __restrict__ part) {
   constexpr int T = 64, R = 16;
   __shared__ float tile[R][kPitch];
   const int split = blockIdx.x / (T / R), band = blockIdx.x % (T / R);
-  const Where w = where<MODE, T>(t, full + split);
+  const Where w = where<GRAM, T>(t, full + split);
   const Mat M = t->m[w.mat];
   const int a = threadIdx.x >> 3, b = (threadIdx.x & 7) * 8;
   float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -482,15 +485,15 @@ __global__ __launch_bounds__(128) void ns_finish64_kernel(const Mats* __restrict
     v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
     v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
   }
-  if (by_rows<MODE>(M)) write8<MODE, true, E>(M, cur, f, v, w.tr * T + band * R + a, w.tc * T + b);
-  if (!by_columns<MODE>(M, w)) return;
+  write8<GRAM, true, float>(M, 0, Coeffs{}, v, w.tr * T + band * R + a, w.tc * T + b);
+  if (w.tr == w.tc) return;
 #pragma unroll
   for (int j = 0; j < 8; ++j) tile[a][b + j] = v[j];
   __syncthreads();
   const int col = threadIdx.x >> 1, r0 = (threadIdx.x & 1) * 8;
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = tile[r0 + j][col];
-  write8<MODE, false, E>(M, cur, f, v, w.tr * T + band * R + r0, w.tc * T + col);
+  write8<GRAM, false, float>(M, 0, Coeffs{}, v, w.tr * T + band * R + r0, w.tc * T + col);
 }
 
 // ------------------------------------------------------------------------------------ host side
@@ -534,7 +537,8 @@ struct Launch {
 };
 
 // The workgroups that the chip holds at a time make a round.  Tiles of whole rounds are not split; those left over may be,
-// into slices of at least 8 stages, where their sums' way through memory costs less than an idle chip.  A stage takes the
+// into slices of at least 8 stages, where their sums' way through memory costs less than an idle chip.  (Of the 64-tiles only
+// X X^T's: the other products' sums over m columns are long enough only where larger tiles are faster.)  A stage takes the
 // variant's time or what the loads of all CUs need for its bytes (measured: 8.7 TB/s, from 128 x 128 tiles on 10.8); a launch
 // has 3.5 us around its stages, and a second round on CUs that hold one workgroup 2.5 of its own.
 Launch launch_with(const List& l, int mode, const Variant& v) {
@@ -554,7 +558,8 @@ Launch launch_with(const List& l, int mode, const Variant& v) {
   const double rounds = (double)(full / round), own = v.per_cu == 1 ? 2.5 : 0.0;
   const double whole = full ? rounds * average * stage(full) + (rounds - (rest ? 0 : 1)) * own : 0.0;
   Launch r = {v, (int)tiles, (int)tiles, 1, 3.5 + whole + (rest ? longest * stage(rest) : 0.0)};
-  for (int64_t S = 2; rest && S <= std::min<int64_t>(round / rest, longest / 8); S += S < 8 ? 1 : 8) {   // (from 8 on by 8: slice k
+  const bool may = rest && (mode == GRAM || v.T > 64);
+  for (int64_t S = 2; may && S <= std::min<int64_t>(round / rest, longest / 8); S += S < 8 ? 1 : 8) {   // (from 8 on by 8: slice k
     // of all tiles on XCD k mod 8, which reads its columns only)
     const double us = 3.5 + whole + (double)longest / S * stage(rest * S) + 4.5 + rest * S * v.T * v.T * 8 / 4e6;
     if (us < r.us) r.full = (int)full, r.S = (int)S, r.us = us;
@@ -572,30 +577,30 @@ Launch launch_of(const List& l, int mode) {
   return best;
 }
 
-template <int MODE, int T, int G, int NS, typename E>
+template <int MODE, int T, int G, int NS, typename ET>
 void product_with(const Launch& r, const Mats* t, int cur, const Coeffs& f, float* part, hipStream_t s) {
-  RL_LAUNCH((ns_product_kernel<MODE, T, G, NS, E>), dim3((unsigned)r.groups()), dim3(Shape<T, G>::threads), 0, s, t, cur, f,
+  RL_LAUNCH((ns_product_kernel<MODE, T, G, NS, ET>), dim3((unsigned)r.groups()), dim3(Shape<T, G>::threads), 0, s, t, cur, f,
             r.full, r.S, part);
   const int split = r.tiles - r.full;
   if (split == 0) return;
-  if constexpr (T == 64)
-    RL_LAUNCH((ns_finish64_kernel<MODE, E>), dim3((unsigned)(split * 4)), dim3(128), 0, s, t, cur, f, r.full, r.S, part);
-  else
-    RL_LAUNCH((ns_finish_kernel<MODE, T, E>), dim3((unsigned)(split * (T / 32) * (T / 32))), dim3(64), 0, s, t, cur, f,
+  if constexpr (T > 64)
+    RL_LAUNCH((ns_finish_kernel<MODE, T, ET>), dim3((unsigned)(split * (T / 32) * (T / 32))), dim3(64), 0, s, t, cur, f,
               r.full, r.S, part);
+  else if constexpr (MODE == GRAM)
+    RL_LAUNCH(ns_finish64_kernel, dim3((unsigned)(split * 4)), dim3(128), 0, s, t, r.full, r.S, part);
 }
 
-template <int MODE, typename E>
+template <int MODE, typename ET>
 void product(const List& l, const Mats* table, int cur, const Coeffs& f, float* part, hipStream_t s) {
   const Launch r = launch_of(l, MODE);
-  if (r.v.T == 256) product_with<MODE, 256, 1, 2, E>(r, table, cur, f, part, s);
-  else if (r.v.T == 128 && r.v.G == 1) product_with<MODE, 128, 1, 2, E>(r, table, cur, f, part, s);
-  else if (r.v.T == 128) product_with<MODE, 128, 2, 4, E>(r, table, cur, f, part, s);
-  else if (r.v.G == 1) product_with<MODE, 64, 1, 4, E>(r, table, cur, f, part, s);
-  else product_with<MODE, 64, 2, 4, E>(r, table, cur, f, part, s);
+  if (r.v.T == 256) product_with<MODE, 256, 1, 2, ET>(r, table, cur, f, part, s);
+  else if (r.v.T == 128 && r.v.G == 1) product_with<MODE, 128, 1, 2, ET>(r, table, cur, f, part, s);
+  else if (r.v.T == 128) product_with<MODE, 128, 2, 4, ET>(r, table, cur, f, part, s);
+  else if (r.v.G == 1) product_with<MODE, 64, 1, 4, ET>(r, table, cur, f, part, s);
+  else product_with<MODE, 64, 2, 4, ET>(r, table, cur, f, part, s);
 }
 
-template <typename E>
+template <typename ET>
 int run(List& l, int steps, const Coeffs& f, double eps, Mats* table, float* part, hipStream_t s) {
   int64_t sum[KINDS] = {};
   for (int i = 0; i < kMats; ++i) {
@@ -606,13 +611,13 @@ int run(List& l, int steps, const Coeffs& f, double eps, Mats* table, float* par
     for (int k = 0; k < 3 && (64 << k) <= l.unit; ++k)
       sum[SYM + k] += tiles_of(m, true, 64 << k), sum[FULL + k] += tiles_of(m, false, 64 << k);
   }
-  RL_LAUNCH((ns_norm_kernel<E>), dim3(kNormBlocks, l.n), dim3(256), 0, s, l.t, table);
-  RL_LAUNCH((ns_load_kernel<E>), dim3((unsigned)sum[LOAD]), dim3(256), 0, s, table, eps);
+  RL_LAUNCH((ns_norm_kernel<ET>), dim3(kNormBlocks, l.n), dim3(256), 0, s, l.t, table);
+  RL_LAUNCH((ns_load_kernel<ET>), dim3((unsigned)sum[LOAD]), dim3(256), 0, s, table, eps);
   for (int k = 0; k < steps; ++k) {
     product<GRAM, float>(l, table, 0, f, part, s);
     product<POLY, float>(l, table, 0, f, part, s);
     if (k + 1 < steps) product<NEXT, float>(l, table, k & 1, f, part, s);
-    else product<LAST, E>(l, table, k & 1, f, part, s);
+    else product<LAST, ET>(l, table, k & 1, f, part, s);
   }
   RL_LAUNCH_CHECK();
   return RLPYT_OK;
@@ -667,6 +672,24 @@ using namespace rlpyt;
 namespace {
 constexpr int64_t kMaxSide = 1 << 16;   // f16 keeps the lo pieces of ~ 1 / sqrt(m n) entries up to here
 
+// Whether the spectral norms of X, A and Q stay in the range of the stored factors: singular values in [0, top] go to
+// |x p(x^2)|, largest at top or where (x p(x^2))' = 0, p(y) = a + b y + c y^2.
+bool stays_bounded(double a, double b, double c, int steps) {
+  const double half = -0.5 * (3.0 * b + copysign(sqrt(9.0 * b * b - 20.0 * a * c), b));
+  const double places[] = {half / (5.0 * c), a / half, -b / (2.0 * c)};    // the last one: p' = 0 (none: NaN or infinite)
+  auto p = [&](double y) { return a + (b + c * y) * y; };
+  double top = 1.0;
+  for (int k = 0; k < steps; ++k) {
+    const double end = top * top;
+    double q = std::max(fabs(a), fabs(p(end))), x = top * fabs(p(end));
+    for (double y : places)
+      if (y > 0.0 && y < end) q = std::max(q, fabs(p(y))), x = std::max(x, sqrt(y) * fabs(p(y)));
+    if (!(fabs(a) < 8.0 && q < 8.0 && x * x < 8.0)) return false;
+    top = x;
+  }
+  return true;
+}
+
 bool sides_ok(const int64_t* rows, const int64_t* cols, int n) {
   for (int i = 0; i < n; ++i)
     if (rows[i] < 0 || cols[i] < 0 || rows[i] > kMaxSide || cols[i] > kMaxSide) return false;
@@ -697,16 +720,8 @@ extern "C" int rlpyt_orthogonalize(int dtype, const void* const* in_host, const 
   if (n == 0) return RLPYT_OK;
   RL_CHECK_ARG(in_host && ld_host && out_host && rows_host && cols_host, RLPYT_EINVAL,
                "rlpyt_orthogonalize: null table");
-  // the spectral norms of X and of the polynomial along the way, from the scalar recurrence on a grid of singular values
-  for (int i = 0; i <= 1024; ++i) {
-    double x = i / 1024.0;
-    for (int k = 0; k < steps; ++k) {
-      const double p = a + (b + c * x * x) * x * x;
-      x *= p;
-      RL_CHECK_ARG(fabs(x) < 8.0 && fabs(p) < 8.0 && x * x < 8.0, RLPYT_EINVAL,
-                   "rlpyt_orthogonalize: coefficients (%g, %g, %g) leave the range of the stored factors", a, b, c);
-    }
-  }
+  RL_CHECK_ARG(stays_bounded(a, b, c, steps), RLPYT_EINVAL,
+               "rlpyt_orthogonalize: coefficients (%g, %g, %g) leave the range of the stored factors", a, b, c);
   RL_CHECK_ARG(sides_ok(rows_host, cols_host, n), RLPYT_ESHAPE,
                "rlpyt_orthogonalize: sides of 0 to %ld are supported", (long)kMaxSide);
   bool any = false;
@@ -737,8 +752,8 @@ extern "C" int rlpyt_orthogonalize(int dtype, const void* const* in_host, const 
     int rc;
     hipStream_t s = (hipStream_t)stream;
     if (dtype == F32) rc = run<float>(l, steps, f, eps, table, part, s);
-    else if (dtype == BF16) rc = run<__bf16>(l, steps, f, eps, table, part, s);
-    else rc = run<_Float16>(l, steps, f, eps, table, part, s);
+    else if (dtype == BF16) rc = run<Bf16>(l, steps, f, eps, table, part, s);
+    else rc = run<Half>(l, steps, f, eps, table, part, s);
     if (rc != RLPYT_OK) return rc;
   }
   return RLPYT_OK;

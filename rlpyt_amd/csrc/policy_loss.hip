@@ -13,7 +13,8 @@
 //
 // Sums over a row are f32 per lane and in a fixed order (no atomics); what is done once per row is in 64 bits, on f32
 // logarithms and exponentials of reduced arguments: kl ~ d^2 / 2 cancels in 32.  Exponents are in base 2 and come from one fma,
-// t = x log2(e) - m with m the rounded product of the largest logit; what that rounding took is put back per row.  -inf
+// t = x log2(e) - m with m the rounded product of the largest logit; what that rounding took is put back per row.  Where m is
+// so large that its rounding could be a large exponent itself (a row of masks), t = (x - largest) log2(e).  -inf
 // logits: t = -inf, e^t = 0, and 0 * t is kept 0 by taking t no lower than -300.  NaN goes through to the loss.
 #include <math.h>
 
@@ -40,7 +41,7 @@ struct LossArgs {
   float *logp, *entropy;          // [N] each, or null
   double* rows;                   // [n, 4]: w pi, w kl, w H, w clipped of a row (or workgroup), or null (log-probabilities only)
   const double* denom;            // sum of valid, or null: N
-  float3* parts;                  // split rows: (max, sum, weighted sum) of the parts [N, P]
+  struct Stats* parts;            // split rows: statistics of the parts [N, P]
   int64_t N, n0, n_rows;          // a launch takes the rows n0 .. n0 + n_rows - 1
   int V, part;                    // part: elements of a row's part, a multiple of 8
   double lo, hi, c_kl, c_ent, g_scale;
@@ -53,16 +54,19 @@ constexpr float kFloor = -300.f;   // 2^-300 is 0 in f32
 __device__ __forceinline__ float exp_of(float t) { return __builtin_amdgcn_exp2f(t); }
 __device__ __forceinline__ float bounded(float t) { return fmaxf(t, kFloor); }
 
-// Softmax statistics of some logits: with t = x log2(e) - m,  s = sum 2^t,  u = sum 2^t t; m = -inf: none.
+// Softmax statistics of some logits: with t = x log2(e) - m,  s = sum 2^t,  u = sum 2^t t; m = -inf: none.  m is a float, the
+// rounded product of the largest logit, up to kFused, and the product itself (48 bits) beyond.
 struct Stats {
-  float m, s, u;
+  double m;
+  float s, u;
 };
+constexpr float kFused = 1 << 20;   // (rounded by 2^-5 at most)
 __device__ __forceinline__ float scaled(float largest) { return largest * kLog2e; }
 __device__ __forceinline__ Stats join(const Stats& p, const Stats& q) {
   Stats r;
-  r.m = fmaxf(p.m, q.m);
+  r.m = fmax(p.m, q.m);
   if (r.m == -INFINITY) return Stats{-INFINITY, p.s + q.s, 0.f};   // (NaN sums stay)
-  const float dp = bounded(p.m - r.m), dq = bounded(q.m - r.m), fp = exp_of(dp), fq = exp_of(dq);
+  const float dp = bounded((float)(p.m - r.m)), dq = bounded((float)(q.m - r.m)), fp = exp_of(dp), fq = exp_of(dq);
   r.s = fmaf(fp, p.s, fq * q.s);
   r.u = fp * fmaf(dp, p.s, p.u) + fq * fmaf(dq, q.s, q.u);
   return r;
@@ -99,24 +103,25 @@ __device__ __forceinline__ double kl_of(double d) {
   return 0.5 * d * d * v;
 }
 
-// What follows from a row's statistics: its terms of the loss, and its gradient as 2^t (k1 t + k0), + ka at the action.
+// What follows from a row's statistics: its terms of the loss, and its gradient as 2^t (k1 t + k0), + ka at the action, with
+// t = (x - base) log2(e) - m, of which one is 0.
 struct RowOut {
   double pi, kl, ent, clipped;
-  float logp, entropy, m, k1, k0, ka;
+  float logp, entropy, base, m, k1, k0, ka;
 };
 __device__ __forceinline__ RowOut row_terms(const LossArgs& p, int64_t n, float w, const Stats& st, float xa,
                                             bool in_range) {
   RowOut o = {};
-  o.m = st.m;
   if (st.m == -INFINITY && st.s == 0.f) {   // every logit is -inf: no distribution, the row adds nothing and has no gradient
-    o.m = 0.f;
     o.logp = -INFINITY;
     return o;
   }
+  if (fabs(st.m) <= (double)kFused) o.m = (float)st.m;
+  else o.base = (float)(st.m / (double)kLog2e);   // (the largest logit again, to its last bit)
   // natural logarithms: x - lse = (x log2(e) - m) ln 2 - log(s)
   const double logs = log_of(st.s), mean = (double)st.u / (double)st.s * kLn2;
   const double H = logs - mean;
-  const double lp = in_range ? ((double)xa * (double)kLog2e - (double)st.m) * kLn2 - logs : (double)NAN;
+  const double lp = in_range ? ((double)xa * (double)kLog2e - st.m) * kLn2 - logs : (double)NAN;
   o.logp = (float)lp;
   o.entropy = (float)H;
   if (!p.rows) return o;
@@ -146,8 +151,9 @@ __device__ __forceinline__ RowOut row_terms(const LossArgs& p, int64_t n, float 
 }
 
 // ---- V <= 4 G: G lanes a row, K elements a lane ---------------------------------------------------------
-template <typename E, int G, int K>
+template <typename ET, int G, int K>
 __global__ __launch_bounds__(256) void loss_group_kernel(const LossArgs p) {
+  typedef typename Elem<ET>::type E;
   __shared__ double sums[4 * 16];
   const int sub = threadIdx.x & (G - 1);
   const int64_t n = p.n0 + (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
@@ -164,13 +170,17 @@ __global__ __launch_bounds__(256) void loss_group_kernel(const LossArgs p) {
       x[k] = live && j < p.V ? (float)row[j] : -INFINITY;
       m = fmaxf(m, x[k]);
     }
-    Stats st = {scaled(group_max<G>(m)), 0.f, 0.f};
-    const float from = st.m == -INFINITY ? 0.f : st.m;
+    m = group_max<G>(m);
+    Stats st = {(double)m * (double)kLog2e, 0.f, 0.f};
+    const float from = m == -INFINITY ? 0.f : m;
+    float e[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const float t = fmaf(x[k], kLog2e, -from), e = exp_of(t);
-      st.s += e;
-      st.u = fmaf(e, bounded(t), st.u);
+      const float t = (x[k] - from) * kLog2e;
+      e[k] = exp_of(t);
+      x[k] = bounded(t);
+      st.s += e[k];
+      st.u = fmaf(e[k], x[k], st.u);
     }
 #pragma unroll
     for (int o2 = G / 2; o2 > 0; o2 >>= 1) {
@@ -189,8 +199,7 @@ __global__ __launch_bounds__(256) void loss_group_kernel(const LossArgs p) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int j = sub + k * G;
-        const float t = fmaf(x[k], kLog2e, -o.m);
-        float v = exp_of(t) * fmaf(o.k1, bounded(t), o.k0);
+        float v = e[k] * fmaf(o.k1, x[k], o.k0);
         if (j == a) v += o.ka;
         if (j < p.V) g[j] = (E)(live ? v : 0.f);
       }
@@ -246,6 +255,16 @@ __device__ __forceinline__ typename Row16<E>::vec grad16(typename Row16<E>::vec 
   for (int k = 0; k < n; ++k) v[k] = (E)g[k];
   return v;
 }
+// Logits of a row whose largest one is beyond kFused, less that one.  (Rounded: nothing where they are near each other, and
+// further away e^t is 0.)
+template <typename E, int R>
+__device__ __forceinline__ void rebase(typename Row16<E>::vec (&x)[R], float base) {
+  if (base == 0.f) return;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int k = 0; k < Row16<E>::n; ++k) x[r][k] = (E)((float)x[r][k] - base);
+}
 // Keeps the compiler from holding the floats of one pass over a row's registers for the next: they are converted again, and
 // two workgroups of 1024 fit a CU, one loading while the other computes.
 template <typename E, int R>
@@ -267,16 +286,26 @@ __device__ __forceinline__ Stats wave_stats(typename Row16<E>::vec (&x)[R]) {
 #pragma unroll
     for (int k = 0; k < n; ++k) m = fmaxf(m, (float)x[r][k]);
   forget<E, R>(x);
-  Stats st = {scaled(group_max<kWave>(m)), 0.f, 0.f};
-  const float from = st.m == -INFINITY ? 0.f : st.m;
+  m = group_max<kWave>(m);
+  Stats st = {(double)scaled(m), 0.f, 0.f};
+  auto add = [&](float t) {
+    const float e = exp_of(t);
+    st.s += e;
+    st.u = fmaf(e, bounded(t), st.u);
+  };
+  if (m == -INFINITY || fabsf(scaled(m)) <= kFused) {
+    const float from = m == -INFINITY ? 0.f : scaled(m);
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int k = 0; k < n; ++k) {
-      const float t = fmaf((float)x[r][k], kLog2e, -from), e = exp_of(t);
-      st.s += e;
-      st.u = fmaf(e, bounded(t), st.u);
-    }
+      for (int k = 0; k < n; ++k) add(fmaf((float)x[r][k], kLog2e, -from));
+  } else {
+    st.m = (double)m * (double)kLog2e;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int k = 0; k < n; ++k) add(((float)x[r][k] - m) * kLog2e);
+  }
   st.s = wave_sum(st.s);
   st.u = wave_sum(st.u);
   return st;
@@ -294,8 +323,9 @@ __device__ __forceinline__ Stats block_join(const Stats& st, Stats* lds) {
   return v;
 }
 
-template <typename E, int NT, int R>
+template <typename ET, int NT, int R>
 __global__ __launch_bounds__(NT) void loss_row_kernel(const LossArgs p) {
+  typedef typename Elem<ET>::type E;
   typedef typename Row16<E>::vec vec;
   constexpr int n16 = Row16<E>::n;
   __shared__ Stats lds[NT / kWave];
@@ -333,6 +363,7 @@ __global__ __launch_bounds__(NT) void loss_row_kernel(const LossArgs p) {
   if (!g) return;
   __syncthreads();
   const RowOut o = out;
+  rebase<E, R>(x, o.base);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int j = (r * NT + threadIdx.x) * n16;
@@ -341,8 +372,9 @@ __global__ __launch_bounds__(NT) void loss_row_kernel(const LossArgs p) {
 }
 
 // ---- a row held by one wave, R x 16 bytes a lane ----------------------------------------------------------
-template <typename E, int R>
+template <typename ET, int R>
 __global__ __launch_bounds__(256) void loss_wave_kernel(const LossArgs p) {
+  typedef typename Elem<ET>::type E;
   typedef typename Row16<E>::vec vec;
   constexpr int n16 = Row16<E>::n;
   __shared__ double sums[4][4];
@@ -364,6 +396,7 @@ __global__ __launch_bounds__(256) void loss_wave_kernel(const LossArgs p) {
     if (lane == 0 && p.logp) p.logp[n] = o.logp, p.entropy[n] = o.entropy;
     if (p.grad) {
       E* g = (E*)p.grad + n * p.V;
+      rebase<E, R>(x, o.base);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const int j = (r * kWave + lane) * n16;
@@ -388,8 +421,9 @@ __global__ __launch_bounds__(256) void loss_wave_kernel(const LossArgs p) {
 // ---- rows split over workgroups ----------------------------------------------------------------------------
 constexpr int kSplitThreads = 256, kSplitVecs = 4;   // vectors in flight per thread
 
-template <typename E>
+template <typename ET>
 __global__ __launch_bounds__(kSplitThreads) void loss_parts_kernel(const LossArgs p, int P) {
+  typedef typename Elem<ET>::type E;
   typedef typename Row16<E>::vec vec;
   constexpr int n16 = Row16<E>::n, step = kSplitThreads * kSplitVecs * n16;
   __shared__ Stats lds[kSplitThreads / kWave];
@@ -406,11 +440,12 @@ __global__ __launch_bounds__(kSplitThreads) void loss_parts_kernel(const LossArg
     st = join(st, wave_stats<E, kSplitVecs>(x));
   }
   st = block_join<kSplitThreads>(st, lds);
-  if (threadIdx.x == 0) p.parts[n * P + i] = float3{st.m, st.s, st.u};
+  if (threadIdx.x == 0) p.parts[n * P + i] = st;
 }
 
-template <typename E>
+template <typename ET>
 __global__ __launch_bounds__(kSplitThreads) void loss_join_kernel(const LossArgs p, int P, int blocks) {
+  typedef typename Elem<ET>::type E;
   typedef typename Row16<E>::vec vec;
   constexpr int n16 = Row16<E>::n, step = kSplitThreads * n16;
   __shared__ Stats lds[kSplitThreads / kWave];
@@ -424,10 +459,7 @@ __global__ __launch_bounds__(kSplitThreads) void loss_join_kernel(const LossArgs
   const E* row = (const E*)p.logits + n * p.row_stride;
   if (live) {
     Stats st = {-INFINITY, 0.f, 0.f};
-    for (int i = threadIdx.x; i < P; i += kSplitThreads) {
-      const float3 q = p.parts[n * P + i];
-      st = join(st, Stats{q.x, q.y, q.z});
-    }
+    for (int i = threadIdx.x; i < P; i += kSplitThreads) st = join(st, p.parts[n * P + i]);
     st = block_join<kSplitThreads>(group_join<kWave>(st), lds);
     if (threadIdx.x == 0) {
       const bool in_range = a >= 0 && a < p.V;
@@ -445,25 +477,34 @@ __global__ __launch_bounds__(kSplitThreads) void loss_join_kernel(const LossArgs
   E* g = (E*)p.grad + n * p.V;
   const int begin = part * p.part, end = min(p.V, begin + p.part);
   for (int j = begin + threadIdx.x * n16; j < end; j += step) {
-    vec v;
+    vec v[1];
     if (live) {
-      v = grad16<E>(load16<E>(row, j, end), j, a, o);
+      v[0] = load16<E>(row, j, end);
+      rebase<E, 1>(v, o.base);
+      v[0] = grad16<E>(v[0], j, a, o);
     } else {
 #pragma unroll
-      for (int k = 0; k < n16; ++k) v[k] = (E)0.f;
+      for (int k = 0; k < n16; ++k) v[0][k] = (E)0.f;
     }
-    store16<E>(g, j, end, v);
+    store16<E>(g, j, end, v[0]);
   }
 }
 
 // ---- sums over the rows -------------------------------------------------------------------------------------
-__global__ __launch_bounds__(1024) void loss_denom_kernel(const float* __restrict__ valid, int64_t N,
-                                                          double* __restrict__ denom) {
-  __shared__ double scratch[16];
-  double v[1] = {0.0};
-  for (int64_t i = threadIdx.x; i < N; i += 1024) v[0] += (double)valid[i];
-  block_sum<1>(v, scratch);
-  if (threadIdx.x == 0) *denom = v[0];
+// One workgroup adds up to kSumRows rows; of more (a million samples took it 0.3 ms) kSumBlocks add a share each, first.
+constexpr int kSumRows = 16384, kSumBlocks = 256;
+
+template <typename T, int K>
+__global__ __launch_bounds__(1024) void loss_sum_kernel(const T* __restrict__ in, int64_t n, double* __restrict__ out) {
+  __shared__ double scratch[K * 16];
+  double v[K] = {};
+#pragma unroll 4
+  for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 1024)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += (double)in[i * K + k];
+  block_sum<K>(v, scratch);
+  if (threadIdx.x == 0)
+    for (int k = 0; k < K; ++k) out[blockIdx.x * K + k] = v[k];
 }
 
 __global__ __launch_bounds__(1024) void loss_finish_kernel(const double* __restrict__ rows, int64_t n,
@@ -472,6 +513,7 @@ __global__ __launch_bounds__(1024) void loss_finish_kernel(const double* __restr
                                                            float* __restrict__ scalars) {
   __shared__ double scratch[4 * 16];
   double v[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 4
   for (int64_t i = threadIdx.x; i < n; i += 1024)
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] += rows[i * 4 + k];
@@ -485,9 +527,11 @@ __global__ __launch_bounds__(1024) void loss_finish_kernel(const double* __restr
 }
 
 // grad *= *scale * factor, in place; nothing is read or written where that is 1 (hence a grid that the chip holds at once).
-template <typename E>
-__global__ __launch_bounds__(256) void loss_scale_kernel(E* __restrict__ g, int64_t n,
+template <typename ET>
+__global__ __launch_bounds__(256) void loss_scale_kernel(void* __restrict__ x, int64_t n,
                                                          const float* __restrict__ scale, float factor) {
+  typedef typename Elem<ET>::type E;
+  E* g = (E*)x;
   typedef typename Row16<E>::vec vec;
   constexpr int n16 = Row16<E>::n;
   const float f = *scale * factor;
@@ -536,33 +580,34 @@ LossPlan plan_of(int64_t N, int64_t V, int size) {
   return q;
 }
 
-template <typename E>
+template <typename ET>
 int run(LossArgs p, const LossPlan& q, hipStream_t s) {
+  typedef typename Elem<ET>::type E;
   const int V = p.V;
   const int64_t vecs = ceil_div((int64_t)V, (int64_t)Row16<E>::n);
   if (V <= kGroupV) {
     const dim3 grid((unsigned)ceil_div(p.n_rows, 256 / group_lanes(V)));
-    if (V <= 8) RL_LAUNCH((loss_group_kernel<E, 8, 1>), grid, dim3(256), 0, s, p);
-    else if (V <= 32) RL_LAUNCH((loss_group_kernel<E, 8, 4>), grid, dim3(256), 0, s, p);
-    else if (V <= 64) RL_LAUNCH((loss_group_kernel<E, 16, 4>), grid, dim3(256), 0, s, p);
-    else RL_LAUNCH((loss_group_kernel<E, 32, 4>), grid, dim3(256), 0, s, p);
+    if (V <= 8) RL_LAUNCH((loss_group_kernel<ET, 8, 1>), grid, dim3(256), 0, s, p);
+    else if (V <= 32) RL_LAUNCH((loss_group_kernel<ET, 8, 4>), grid, dim3(256), 0, s, p);
+    else if (V <= 64) RL_LAUNCH((loss_group_kernel<ET, 16, 4>), grid, dim3(256), 0, s, p);
+    else RL_LAUNCH((loss_group_kernel<ET, 32, 4>), grid, dim3(256), 0, s, p);
   } else if (V * (int64_t)sizeof(E) <= kWaveBytes) {
     const dim3 grid((unsigned)ceil_div(p.n_rows, 4));
-    if (vecs <= 64) RL_LAUNCH((loss_wave_kernel<E, 1>), grid, dim3(256), 0, s, p);
-    else if (vecs <= 128) RL_LAUNCH((loss_wave_kernel<E, 2>), grid, dim3(256), 0, s, p);
-    else RL_LAUNCH((loss_wave_kernel<E, 4>), grid, dim3(256), 0, s, p);
+    if (vecs <= 64) RL_LAUNCH((loss_wave_kernel<ET, 1>), grid, dim3(256), 0, s, p);
+    else if (vecs <= 128) RL_LAUNCH((loss_wave_kernel<ET, 2>), grid, dim3(256), 0, s, p);
+    else RL_LAUNCH((loss_wave_kernel<ET, 4>), grid, dim3(256), 0, s, p);
   } else if (q.P == 0) {
     const dim3 grid((unsigned)p.n_rows);
-    if (vecs <= 512) RL_LAUNCH((loss_row_kernel<E, 256, 2>), grid, dim3(256), 0, s, p);
-    else if (vecs <= 1024) RL_LAUNCH((loss_row_kernel<E, 256, 4>), grid, dim3(256), 0, s, p);
-    else if (vecs <= 2048) RL_LAUNCH((loss_row_kernel<E, 512, 4>), grid, dim3(512), 0, s, p);
-    else if (vecs <= 4096) RL_LAUNCH((loss_row_kernel<E, 1024, 4>), grid, dim3(1024), 0, s, p);
-    else if (vecs <= 8192) RL_LAUNCH((loss_row_kernel<E, 1024, 8>), grid, dim3(1024), 0, s, p);
-    else RL_LAUNCH((loss_row_kernel<E, 1024, 16>), grid, dim3(1024), 0, s, p);
+    if (vecs <= 512) RL_LAUNCH((loss_row_kernel<ET, 256, 2>), grid, dim3(256), 0, s, p);
+    else if (vecs <= 1024) RL_LAUNCH((loss_row_kernel<ET, 256, 4>), grid, dim3(256), 0, s, p);
+    else if (vecs <= 2048) RL_LAUNCH((loss_row_kernel<ET, 512, 4>), grid, dim3(512), 0, s, p);
+    else if (vecs <= 4096) RL_LAUNCH((loss_row_kernel<ET, 1024, 4>), grid, dim3(1024), 0, s, p);
+    else if (vecs <= 8192) RL_LAUNCH((loss_row_kernel<ET, 1024, 8>), grid, dim3(1024), 0, s, p);
+    else RL_LAUNCH((loss_row_kernel<ET, 1024, 16>), grid, dim3(1024), 0, s, p);
   } else {
     const int blocks = p.grad ? q.P : 1;
-    RL_LAUNCH((loss_parts_kernel<E>), dim3((unsigned)(p.n_rows * q.P)), dim3(kSplitThreads), 0, s, p, q.P);
-    RL_LAUNCH((loss_join_kernel<E>), dim3((unsigned)(p.n_rows * blocks)), dim3(kSplitThreads), 0, s, p, q.P, blocks);
+    RL_LAUNCH((loss_parts_kernel<ET>), dim3((unsigned)(p.n_rows * q.P)), dim3(kSplitThreads), 0, s, p, q.P);
+    RL_LAUNCH((loss_join_kernel<ET>), dim3((unsigned)(p.n_rows * blocks)), dim3(kSplitThreads), 0, s, p, q.P, blocks);
   }
   RL_LAUNCH_CHECK();
   return RLPYT_OK;
@@ -579,15 +624,16 @@ int run_all(int dtype, LossArgs p, const LossPlan& q, hipStream_t s) {
     p.n_rows = std::min(slice, p.N - p.n0);
     int rc;
     if (dtype == F32) rc = run<float>(p, q, s);
-    else if (dtype == BF16) rc = run<__bf16>(p, q, s);
-    else rc = run<_Float16>(p, q, s);
+    else if (dtype == BF16) rc = run<Bf16>(p, q, s);
+    else rc = run<Half>(p, q, s);
     if (rc != RLPYT_OK) return rc;
   }
   return RLPYT_OK;
 }
 
-// workspace: sum of valid | 4 partial sums per row or workgroup | statistics of the parts
-int64_t parts_offset(const LossPlan& q) { return 16 + q.partials * 4 * (int64_t)sizeof(double); }
+// workspace: sum of valid | sums of shares | 4 partial sums per row or workgroup | statistics of the parts
+constexpr int64_t kRowsOffset = 16 + kSumBlocks * 4 * (int64_t)sizeof(double);
+int64_t parts_offset(const LossPlan& q) { return kRowsOffset + q.partials * 4 * (int64_t)sizeof(double); }
 
 }  // namespace
 }  // namespace rlpyt
@@ -595,9 +641,9 @@ int64_t parts_offset(const LossPlan& q) { return 16 + q.partials * 4 * (int64_t)
 using namespace rlpyt;
 
 extern "C" int64_t rlpyt_policy_loss_workspace_bytes(int dtype, int64_t N, int64_t V) {
-  if (dtype < F32 || dtype > F16 || N <= 0 || V <= 0) return 16;
+  if (dtype < F32 || dtype > F16 || N <= 0 || V <= 0) return kRowsOffset;
   const LossPlan q = plan_of(N, V, element_size(dtype));
-  return parts_offset(q) + N * q.P * (int64_t)sizeof(float3);
+  return parts_offset(q) + N * q.P * (int64_t)sizeof(Stats);
 }
 
 extern "C" int rlpyt_policy_kl_loss_fwd_bwd(int dtype, const void* logits, int64_t row_stride,
@@ -617,17 +663,28 @@ extern "C" int rlpyt_policy_kl_loss_fwd_bwd(int dtype, const void* logits, int64
   LossArgs p = {};
   p.logits = logits, p.row_stride = row_stride, p.action = action, p.old_logp = old_logp, p.advantage = advantage;
   p.ref_logp = ref_logp, p.valid = valid, p.grad = grad;
-  double* denom = (double*)workspace;
-  p.rows = (double*)((char*)workspace + 16);
+  double *denom = (double*)workspace, *shares = (double*)((char*)workspace + 16);
+  p.rows = (double*)((char*)workspace + kRowsOffset);
   p.denom = valid ? denom : nullptr;
-  p.parts = (float3*)((char*)workspace + parts_offset(q));
+  p.parts = (Stats*)((char*)workspace + parts_offset(q));
   p.N = N, p.V = (int)V, p.part = q.part;
   p.lo = clip_low, p.hi = clip_high, p.c_kl = kl_coeff, p.c_ent = entropy_coeff, p.g_scale = grad_scale;
-  if (valid) RL_LAUNCH(loss_denom_kernel, dim3(1), dim3(1024), 0, s, valid, N, denom);
+  if (valid && N > kSumRows) {
+    RL_LAUNCH((loss_sum_kernel<float, 1>), dim3(kSumBlocks), dim3(1024), 0, s, valid, N, shares);
+    RL_LAUNCH((loss_sum_kernel<double, 1>), dim3(1), dim3(1024), 0, s, shares, kSumBlocks, denom);
+  } else if (valid) {
+    RL_LAUNCH((loss_sum_kernel<float, 1>), dim3(1), dim3(1024), 0, s, valid, N, denom);
+  }
   const int rc = run_all(dtype, p, q, s);
   if (rc != RLPYT_OK) return rc;
-  RL_LAUNCH(loss_finish_kernel, dim3(1), dim3(1024), 0, s, p.rows, N ? q.partials : 0, p.denom, (double)N, kl_coeff,
-            entropy_coeff, loss, scalars);
+  const double* rows = p.rows;
+  int64_t sums = N ? q.partials : 0;
+  if (sums > kSumRows) {
+    RL_LAUNCH((loss_sum_kernel<double, 4>), dim3(kSumBlocks), dim3(1024), 0, s, rows, sums, shares);
+    rows = shares, sums = kSumBlocks;
+  }
+  RL_LAUNCH(loss_finish_kernel, dim3(1), dim3(1024), 0, s, rows, sums, p.denom, (double)N, kl_coeff, entropy_coeff, loss,
+            scalars);
   RL_LAUNCH_CHECK();
   return RLPYT_OK;
 }
@@ -643,7 +700,7 @@ extern "C" int rlpyt_action_logp(int dtype, const void* logits, int64_t row_stri
   const LossPlan q = plan_of(N, V, element_size(dtype));
   LossArgs p = {};
   p.logits = logits, p.row_stride = row_stride, p.action = action, p.logp = logp, p.entropy = entropy;
-  p.parts = (float3*)((char*)workspace + parts_offset(q));
+  p.parts = (Stats*)((char*)workspace + parts_offset(q));
   p.N = N, p.V = (int)V, p.part = q.part;
   return run_all(dtype, p, q, (hipStream_t)stream);
 }
@@ -658,9 +715,9 @@ extern "C" int rlpyt_scale_unless_one(int dtype, void* x, int64_t n, const float
   hipStream_t s = (hipStream_t)stream;
   const int per = 256 * (16 / element_size(dtype));
   const dim3 grid((unsigned)std::min<int64_t>(1024, ceil_div(n, per)));
-  if (dtype == F32) RL_LAUNCH((loss_scale_kernel<float>), grid, dim3(256), 0, s, (float*)x, n, scale, factor);
-  else if (dtype == BF16) RL_LAUNCH((loss_scale_kernel<__bf16>), grid, dim3(256), 0, s, (__bf16*)x, n, scale, factor);
-  else RL_LAUNCH((loss_scale_kernel<_Float16>), grid, dim3(256), 0, s, (_Float16*)x, n, scale, factor);
+  if (dtype == F32) RL_LAUNCH((loss_scale_kernel<float>), grid, dim3(256), 0, s, x, n, scale, factor);
+  else if (dtype == BF16) RL_LAUNCH((loss_scale_kernel<Bf16>), grid, dim3(256), 0, s, x, n, scale, factor);
+  else RL_LAUNCH((loss_scale_kernel<Half>), grid, dim3(256), 0, s, x, n, scale, factor);
   RL_LAUNCH_CHECK();
   return RLPYT_OK;
 }

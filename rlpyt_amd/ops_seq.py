@@ -63,7 +63,8 @@ def gated_scan(x, gate, h0=None, reset=None, lengths=None):
     Differentiable w.r.t. ``x``, ``gate`` and ``h0`` (once).
 
     ``x, gate``: float32, bfloat16 or float16, any strides along time and batch (a ``[B, T, D]`` tensor goes
-    in as its ``transpose(0, 1)``, the halves of one projection as its ``chunk(2, -1)``); up to 2^28 channels ``B D``.
+    in as its ``transpose(0, 1)``, the halves of one projection as its ``chunk(2, -1)``); up to 2^28 channels ``B D``
+    and less than 2^30 steps.
     ``h0 [B, D]``: the state before the first step (None: 0); other floating types are converted to float32.
     ``reset [T, B]`` (bool, uint8 or nonzero float, as ``done``): the state is cleared BEFORE step t, whatever it
     held.  ``lengths [B]`` (integers, clamped to 0 .. T): steps from ``lengths[b]`` on are not part of sequence b:
@@ -74,6 +75,8 @@ def gated_scan(x, gate, h0=None, reset=None, lengths=None):
     if x.dim() != 3 or x.shape != gate.shape:
         _refuse(f"gated_scan: x and gate [T, B, D] are needed, got {tuple(x.shape)} and {tuple(gate.shape)}")
     T, B, D = x.shape
+    if T >= 1 << 30 or B * D > 1 << 28:
+        _refuse(f"gated_scan: less than 2^30 steps and up to 2^28 channels are supported, got {tuple(x.shape)}")
     if x.dtype not in _DTYPES or gate.dtype != x.dtype:
         _refuse(f"gated_scan: x and gate of one type, float32, bfloat16 or float16, are needed, got {x.dtype} "
                 f"and {gate.dtype}")
@@ -109,6 +112,8 @@ def gated_scan_step(x, gate, state, reset=None):
     if x.dtype not in _DTYPES or gate.dtype != x.dtype:
         _refuse(f"gated_scan_step: x and gate of one type, float32, bfloat16 or float16, are needed, got {x.dtype} "
                 f"and {gate.dtype}")
+    if shape[0] * shape[1] > 1 << 28:
+        _refuse(f"gated_scan_step: up to 2^28 channels are supported, got {tuple(shape)}")
     if state.shape != shape or state.dtype != torch.float32 or not state.is_contiguous():
         _refuse("gated_scan_step: state has to be a dense float32 [B, D]")
     if reset is not None and reset.shape != shape[:1]:
@@ -132,7 +137,7 @@ def gated_scan_step(x, gate, state, reset=None):
 def _logit_rows(name, logits, action):
     """The rows ``[N, V]`` of ``logits [..., V]`` with unit stride along V (a view where the strides allow one), and the
     flat int64 actions."""
-    if logits.dim() < 1 or logits.shape[-1] == 0 or logits.dtype not in _DTYPES:
+    if logits.dim() < 1 or not 0 < logits.shape[-1] <= 1 << 30 or logits.dtype not in _DTYPES:
         _refuse(f"{name}: logits [..., V] in float32, bfloat16 or float16 are needed, got {tuple(logits.shape)} "
                 f"{logits.dtype}")
     if action.shape != logits.shape[:-1] or action.is_floating_point() or action.dtype == torch.bool:
@@ -233,6 +238,8 @@ def orthogonalize(mats, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     for g in mats:
         if g.dim() < 2 or g.dtype not in _DTYPES:
             _refuse(f"orthogonalize: matrices in float32, bfloat16 or float16 are needed, got {tuple(g.shape)} {g.dtype}")
+        if max(g.shape[-2:]) > 1 << 16:
+            _refuse(f"orthogonalize: sides up to 65536 are supported, got {tuple(g.shape)}")
     if not mats:
         return []
     _need_device("orthogonalize", *mats)

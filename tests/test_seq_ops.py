@@ -47,6 +47,12 @@ z = torch.zeros
     lambda: ops.orthogonalize(z(4, 4), steps=2.5),
     lambda: ops.orthogonalize(z(4, 4), coeffs=(1., 2.)),
     lambda: ops.orthogonalize(z(4, 4), eps=-1.),
+    lambda: ops.gated_scan(z(1, 1, 1).expand(1, 1 << 15, 1 << 14), z(1, 1, 1).expand(1, 1 << 15, 1 << 14)),
+    lambda: ops.gated_scan(z(1, 1, 1).expand(1 << 30, 1, 1), z(1, 1, 1).expand(1 << 30, 1, 1)),
+    lambda: ops.gated_scan_step(z(1, 1).expand(1 << 15, 1 << 14), z(1, 1).expand(1 << 15, 1 << 14), z(1, 1)),
+    lambda: ops.policy_kl_loss(z(1, 1).expand(1, (1 << 30) + 1), z(1).long(), z(1), z(1)),
+    lambda: ops.action_logp(z(1, 1).expand(1, (1 << 30) + 1), z(1).long()),
+    lambda: ops.orthogonalize(z(1, 1).expand(1, (1 << 16) + 1)),
     lambda: Muon([z(3, 3, requires_grad=True)], lr=-1.),
     lambda: Muon([z(3, 3, requires_grad=True)], momentum=1.),
 ])

@@ -474,6 +474,52 @@ def test_policy_kl_loss_far_logits_and_ratios():
     assert abs(float(loss) + 1.3 * 0.5) < 1e-6 and not bool(grad.any())
 
 
+def test_policy_kl_loss_sums_over_many_rows(N=20000, V=200):
+    # more rows than one workgroup adds: shares first.  (Sums over rows are 64 bits, so the tolerances do not grow.)
+    data = loss_data(N, V, torch.float32, 52)
+    c = dict(kl_coeff=0.1, entropy_coeff=0.02)
+    logits, action, old, adv, ref, w = data
+    # a row's gradient is w / sum w times p or 1 - p times the sum of -r A, -0.1 (e^d - 1) and 0.02 (log p + H): with log p known
+    # to err, r and e^d are to err relative; in some of many rows the three cancel to less than err of their sizes
+    lp = torch.log_softmax(logits.double(), -1).gather(-1, action[:, None]).squeeze(-1)
+    parts = (lp - old).exp() * adv.abs() + 0.1 * ((ref - lp).exp() + 1.) + 0.02 * math.log(V)
+    loss_close(*run_loss(*data, **KW, **c), *loss64(logits, action, old, adv, ref, w, 0.2, 0.3, 0.1, 0.02),
+               cancel=(parts * w / w.double().sum())[:, None])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("V", [5, 30, 100, 900, 3500, 40000])
+def test_policy_kl_loss_of_huge_logits(V, dtype):
+    """Masks of the type's lowest value and others, also over whole rows, are logits like all others: a row of equal ones is
+    uniform.  2^20 ln 2 = 726817 is where another expression takes over."""
+    N, least, most = 10, torch.finfo(dtype).min, torch.finfo(dtype).max
+    noise = torch.randn(N, V, device=DEV, generator=gen(55)).double()
+    logits = torch.zeros(N, V, device=DEV, dtype=torch.float64)
+    logits[0], logits[1], logits[2], logits[3] = least, -1e30, most, 1e30
+    logits[4] = least
+    logits[4, V // 2] = 0.5
+    logits[5] = -1e9 + 100. * noise[5]
+    logits[6], logits[7] = 726817. + noise[6], -726817. + noise[7]
+    logits[8] = least
+    logits[8, ::2] = -math.inf
+    logits[9] = noise[9]
+    logits[9, 1::2] = least
+    logits = logits.clamp(least, most).masked_fill(logits == -math.inf, -math.inf).to(dtype)
+    action = logits.argmax(-1)
+    l64 = torch.log_softmax(logits.double(), -1)
+    want = l64.gather(-1, action[:, None]).squeeze(-1)
+    lp, ent = ops.action_logp(logits, action)
+    tol = 2. ** -20 + 68 * 2. ** -24               # as in test_policy_kl_loss
+    assert bool(((lp.double() - want).abs() <= tol + want.abs() * 2. ** -24).all()), (lp, want)
+    want_ent = -(l64.exp() * l64.clamp(min=-1e300)).sum(-1)
+    assert bool(((ent.double() - want_ent).abs() <= tol * (1 + want_ent)).all()), (ent, want_ent)
+    g = gen(56)
+    old, ref = (want + 0.1 * torch.rand(N, device=DEV, generator=g)).float(), (want + 0.2).float()
+    adv = torch.randn(N, device=DEV, generator=g)
+    out = run_loss(logits, action, old, adv, ref, None, kl_coeff=0.1, **KW)
+    loss_close(*out, *loss64(logits, action, old, adv, ref, None, 0.2, 0.3, 0.1))
+
+
 def test_policy_kl_loss_gradient_against_differences():
     logits, action, old, adv, ref, w = loss_data(40, 300, torch.float32, 60)
     c = dict(kl_coeff=0.3, entropy_coeff=0.2)
@@ -647,6 +693,9 @@ def test_orthogonalize_options_and_edges():
     bad = g.clone()
     bad[3, 4] = float("nan")
     assert bool(torch.isnan(ops.orthogonalize(bad)).any())
+    for size in (1e-36, 1e36):               # a reciprocal norm beyond 32 bits
+        orth_close(ops.orthogonalize(g * size, eps=0.), orth64(g * size, eps=0.))
+    assert not bool(ops.orthogonalize(torch.zeros(30, 20, device=DEV), eps=0.).any())
     low = g[:, :1] @ g[:1, :]                # rank 1: the noise of the products is amplified 484 times
     got, want = ops.orthogonalize(low), orth64(low)
     assert float((got.double() - want).norm()) <= 484 * 2. ** -22 * 4 * float(want.norm())

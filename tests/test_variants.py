@@ -811,6 +811,113 @@ def _sumtree_input_priorities():
     P.test_sumtree_streams_bit_exact(_ops(), "inpri")
 
 
+# ----------------------------------------------------------------------- sequence operators
+# (data, 64-bit formulas and tolerances are test_seq_ops_gpu's)
+SEQ_TYPES = {"float": torch.float32, "Bf16": torch.bfloat16, "Half": torch.float16}
+
+
+def _gated_scan_case(dtype, D, reset, lengths):
+    def run():
+        import test_seq_ops_gpu as P
+        T = 600                          # few channels: cut into segments, reduced first (the last flag)
+        x, gate, h0, dh, dhn, rs, ln = data = P.scan_data(T, 3, D, dtype, 31, reset, lengths)
+        P.scan_close(P.scan_grads(*data), P.scan64(x, gate, h0, rs, ln, dh, dhn), T)
+    return run
+
+
+for _e, _t in SEQ_TYPES.items():
+    for _v in ((1,) if _e == "float" else (1, 2)):
+        for _r, _l in ((0, 0), (0, 1), (1, 0), (1, 1)):
+            case(*[f"gated_scan_{d}_kernel<{_e}, {_v}, {str(bool(_r)).lower()}, {str(bool(_l)).lower()}, {agg}>"
+                   for d in ("fwd", "bwd") for agg in ("false", "true")])(
+                _gated_scan_case(_t, 130 if _v == 2 else 70 if _e == "float" else 1, _r, _l))
+
+
+def _gated_scan_step_case(dtype, D):
+    def run():
+        import test_seq_ops_gpu as P
+        P.test_gated_scan_step_is_one_step_of_the_scan((7, D), dtype)
+    return run
+
+
+for _e, _t in SEQ_TYPES.items():
+    case(f"gated_scan_step_kernel<{_e}, 1>")(_gated_scan_step_case(_t, 65))
+    case(f"gated_scan_step_kernel<{_e}, 2>")(_gated_scan_step_case(_t, 130))
+
+
+def _policy_loss_case(dtype, N, V):
+    def run():
+        import test_seq_ops_gpu as P
+        P.test_policy_kl_loss((N, V), dtype)
+    return run
+
+
+for _e, _t in SEQ_TYPES.items():
+    _n = 2 if _e == "float" else 4       # thousands of elements in 8 KB
+    for _k, _v in (("8, 1", 7), ("8, 4", 20), ("16, 4", 50), ("32, 4", 100)):
+        case(f"loss_group_kernel<{_e}, {_k}>")(_policy_loss_case(_t, 37, _v))
+    for _k, _v in ((1, 100), (2, 200), (4, 500)):
+        case(f"loss_wave_kernel<{_e}, {_k}>")(_policy_loss_case(_t, 37, _n * _v + 1))
+    for _k, _v in (("256, 2", 750), ("256, 4", 1750), ("512, 4", 3500), ("1024, 4", 7500), ("1024, 8", 15000),
+                   ("1024, 16", 30000)):
+        case(f"loss_row_kernel<{_e}, {_k}>")(_policy_loss_case(_t, 256, _n * _v + 1))
+    case(f"loss_parts_kernel<{_e}>", f"loss_join_kernel<{_e}>")(_policy_loss_case(_t, 3, 70001))
+
+
+@case("loss_finish_kernel", "loss_sum_kernel<float, 1>", "loss_sum_kernel<double, 1>", "loss_sum_kernel<double, 4>")
+def _policy_loss_sums():
+    import test_seq_ops_gpu as P
+    P.test_policy_kl_loss_sums_over_many_rows(600000, 3)
+
+
+def _policy_loss_scale_case(dtype):
+    def run():
+        import test_seq_ops_gpu as P
+        logits, action, old, adv, ref, w = P.loss_data(9, 50, dtype, 20)
+        leaf = logits.clone().requires_grad_(True)
+        loss, _ = _ops().policy_kl_loss(leaf, action, old, adv, valid=w)
+        plain, = torch.autograd.grad(loss, leaf)
+        loss, _ = _ops().policy_kl_loss(leaf, action, old, adv, valid=w)
+        twice, = torch.autograd.grad(2. * loss, leaf)
+        assert bool(plain.any()) and torch.equal(twice, 2. * plain)
+    return run
+
+
+for _e, _t in SEQ_TYPES.items():
+    case(f"loss_scale_kernel<{_e}>")(_policy_loss_scale_case(_t))
+
+
+def _orthogonalize_case(dtype, m, n, count):
+    def run():
+        import test_seq_ops_gpu as P
+        g = torch.randn(count, m, n, device="cuda", generator=P.gen(95)).to(dtype)
+        for got, mat in zip(_ops().orthogonalize(g, steps=2), g):
+            P.orth_close(got, P.orth64(mat, steps=2))
+    return run
+
+
+# which products the sizes take: tiles, sets of waves; "f": and split over their sums
+for _size, _products in (((16, 16, 1), "0,64,2 1,64,2 2,64,2"),
+                         ((16, 2200, 8), "0,64,2f 2,64,1"),
+                         ((200, 200, 32), "0,64,1 1,64,1"),
+                         ((400, 512, 16), "0,128,2 1,128,2 2,128,2"),
+                         ((1600, 1600, 1), "0,128,1f 1,128,1f 2,128,1f"),
+                         ((2500, 2500, 16), "0,256,1f 1,256,1f 2,256,1f")):
+    for _e, _t in SEQ_TYPES.items():
+        _names = []
+        for _p in _products.split():
+            _mode, _tile, _sets = _p.rstrip("f").split(",")
+            _stages = {"64": 4, "128": 2 * int(_sets), "256": 2}[_tile]
+            _args = [(_mode, "float")] + ([("3", _e)] if _mode == "2" else [])    # (3: the last step's, in the output's type)
+            for _m, _out in _args:
+                _names.append(f"ns_product_kernel<{_m}, {_tile}, {_sets}, {_stages}, {_out}>")
+                if _p.endswith("f"):
+                    _names.append("ns_finish64_kernel" if _tile == "64" else f"ns_finish_kernel<{_m}, {_tile}, {_out}>")
+        if _size == (16, 16, 1):
+            _names += [f"ns_norm_kernel<{_e}>", f"ns_load_kernel<{_e}>"]
+        case(*[n for n in _names if n not in CASES])(_orthogonalize_case(_t, *_size))
+
+
 # ===================================================================================== tests
 def test_every_kernel_instantiation_has_a_parity_case():
     """CPU: the case table and the library agree (no unnamed kernel, no stale entry)."""
