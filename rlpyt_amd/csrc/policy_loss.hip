@@ -150,67 +150,90 @@ __device__ __forceinline__ RowOut row_terms(const LossArgs& p, int64_t n, float 
   return o;
 }
 
-// ---- V <= 4 G: G lanes a row, K elements a lane ---------------------------------------------------------
-template <typename ET, int G, int K>
+// ---- V <= K G: G lanes a row, K elements a lane, R rows one after the other ---------------------------------
+// What is done once per row is ~150 operations in 64 bits, as much as the rest of 50 elements: lane r of a group does row r's.
+// Joins the values of G lanes (8 or 16) within the vector unit, lane permutations as operands; every lane gets the result.
+template <int CTRL>
+__device__ __forceinline__ float permuted(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int G, typename F>
+__device__ __forceinline__ float joined(float v, F f) {
+  v = f(v, permuted<0xb1>(v));               // lanes 1 0 3 2
+  v = f(v, permuted<0x4e>(v));               // lanes 2 3 0 1
+  v = f(v, permuted<0x141>(v));              // 8 lanes mirrored
+  if (G == 16) v = f(v, permuted<0x140>(v));   // 16 lanes mirrored
+  return v;
+}
+
+template <typename ET, int G, int K, int R>
 __global__ __launch_bounds__(256) void loss_group_kernel(const LossArgs p) {
   typedef typename Elem<ET>::type E;
+  constexpr int each = 256 / G;           // groups of a workgroup, and rows of a round
   __shared__ double sums[4 * 16];
   const int sub = threadIdx.x & (G - 1);
-  const int64_t n = p.n0 + (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
-  const bool on = n < p.n0 + p.n_rows;
-  const float w = on ? (p.valid ? p.valid[n] : 1.f) : 0.f;
-  RowOut o = {};
-  if (on) {
-    const bool live = w != 0.f;           // padded rows are not read
-    const E* row = (const E*)p.logits + n * p.row_stride;
-    float x[K], m = -INFINITY;
+  const int64_t first = p.n0 + (int64_t)blockIdx.x * (each * R) + threadIdx.x / G, end = p.n0 + p.n_rows;
+  const int64_t own = first + sub * each;    // the row whose terms this lane works out
+  const bool mine = sub < R && own < end;
+  const float w = mine ? (p.valid ? p.valid[own] : 1.f) : 0.f;
+  const int64_t action = w != 0.f ? p.action[own] : -1;
+  const bool in_range = action >= 0 && action < p.V;
+  const float xa = in_range ? (float)((const E*)p.logits)[own * p.row_stride + action] : 0.f;
+  float t[R][K];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const bool live = __shfl(w, r, G) != 0.f;   // padded rows are not read
+    const E* row = (const E*)p.logits + (first + r * each) * p.row_stride;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int j = sub + k * G;
-      x[k] = live && j < p.V ? (float)row[j] : -INFINITY;
-      m = fmaxf(m, x[k]);
+      t[r][k] = live && j < p.V ? (float)row[j] : -INFINITY;
     }
-    m = group_max<G>(m);
-    Stats st = {(double)m * (double)kLog2e, 0.f, 0.f};
+  }
+  Stats st = {-INFINITY, 0.f, 0.f};
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float m = t[r][0], s = 0.f, u = 0.f;
+#pragma unroll
+    for (int k = 1; k < K; ++k) m = fmaxf(m, t[r][k]);
+    m = joined<G>(m, [](float a, float b) { return fmaxf(a, b); });
     const float from = m == -INFINITY ? 0.f : m;
-    float e[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const float t = (x[k] - from) * kLog2e;
-      e[k] = exp_of(t);
-      x[k] = bounded(t);
-      st.s += e[k];
-      st.u = fmaf(e[k], x[k], st.u);
+      const float x = (t[r][k] - from) * kLog2e, e = exp_of(x);
+      t[r][k] = bounded(x);
+      s += e;
+      u = fmaf(e, t[r][k], u);
     }
+    s = joined<G>(s, [](float a, float b) { return a + b; });
+    u = joined<G>(u, [](float a, float b) { return a + b; });
+    if (sub == r) st = Stats{(double)m * (double)kLog2e, s, u};
+  }
+  RowOut o = {};
+  if (w != 0.f) {
+    o = row_terms(p, own, w, st, xa, in_range);
+    if (p.logp) p.logp[own] = o.logp, p.entropy[own] = o.entropy;
+  }
+  if (p.grad) {
 #pragma unroll
-    for (int o2 = G / 2; o2 > 0; o2 >>= 1) {
-      st.s += __shfl_xor(st.s, o2, kWave);
-      st.u += __shfl_xor(st.u, o2, kWave);
-    }
-    if (live) {
-      const int64_t a = p.action[n];
-      const bool in_range = a >= 0 && a < p.V;
-      o = row_terms(p, n, w, st, in_range ? (float)row[a] : 0.f, in_range);
-      if (p.logp && sub == 0) p.logp[n] = o.logp, p.entropy[n] = o.entropy;
-    }
-    if (p.grad) {
-      E* g = (E*)p.grad + n * p.V;
-      const int64_t a = live ? p.action[n] : -1;
+    for (int r = 0; r < R; ++r) {
+      const float k1 = __shfl(o.k1, r, G), k0 = __shfl(o.k0, r, G), ka = __shfl(o.ka, r, G);
+      const int a = __shfl(in_range ? (int)action : -1, r, G);
+      E* g = (E*)p.grad + (first + r * each) * p.V;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int j = sub + k * G;
-        float v = e[k] * fmaf(o.k1, x[k], o.k0);
-        if (j == a) v += o.ka;
-        if (j < p.V) g[j] = (E)(live ? v : 0.f);
+        float v = exp_of(t[r][k]) * fmaf(k1, t[r][k], k0);   // (2^-300 is 0 too)
+        if (j == a) v += ka;
+        if (j < p.V && first + r * each < end) g[j] = (E)v;
       }
     }
   }
   if (!p.rows) return;
-  double v[4] = {0.0, 0.0, 0.0, 0.0};
-  if (sub == 0) v[0] = o.pi, v[1] = o.kl, v[2] = o.ent, v[3] = o.clipped;
+  double v[4] = {o.pi, o.kl, o.ent, o.clipped};
   block_sum<4>(v, sums);
   if (threadIdx.x == 0)
-    for (int k = 0; k < 4; ++k) p.rows[(p.n0 / (256 / G) + blockIdx.x) * 4 + k] = v[k];
+    for (int k = 0; k < 4; ++k) p.rows[(p.n0 / (each * R) + blockIdx.x) * 4 + k] = v[k];
 }
 
 // ---- a row held by one workgroup of NT threads, R x 16 bytes a thread -------------------------------------
@@ -557,14 +580,17 @@ struct LossPlan {
   int P, part;                      // P > 0: rows split into P parts of `part` elements
   int64_t partials;                 // rows of the [., 4] table of partial sums
 };
-int group_lanes(int64_t V) { return V <= 32 ? 8 : V <= 64 ? 16 : 32; }
+int group_lanes(int64_t V) { return V <= 32 ? 8 : 16; }
+// Rows of a group.  262144 x 18 in f32 takes 49 us by one row each and 35 by four, 8192 x 18 18.4 and 19.1 (fewer
+// workgroups, and what a lane does for a row is not hidden behind others).
+int group_rows(int64_t N) { return N >= 32768 ? 4 : 1; }
 
 // A row goes to a group of lanes, a wave or a workgroup (256 KB at most) whose registers hold it, while the rows fill the chip;
 // otherwise it is split into parts of at least 8 KB so that there are about 1024 workgroups.
 LossPlan plan_of(int64_t N, int64_t V, int size) {
   LossPlan q = {0, 0, N};
   if (V <= kGroupV) {
-    q.partials = ceil_div(N, 256 / group_lanes(V));
+    q.partials = ceil_div(N, 256 / group_lanes(V) * group_rows(N));
     return q;
   }
   if (V * size <= kWaveBytes) {
@@ -580,17 +606,24 @@ LossPlan plan_of(int64_t N, int64_t V, int size) {
   return q;
 }
 
+template <typename ET, int R>
+void launch_groups(const LossArgs& p, hipStream_t s) {
+  const int V = p.V;
+  const dim3 grid((unsigned)ceil_div(p.n_rows, 256 / group_lanes(V) * R));
+  if (V <= 8) RL_LAUNCH((loss_group_kernel<ET, 8, 1, R>), grid, dim3(256), 0, s, p);
+  else if (V <= 32) RL_LAUNCH((loss_group_kernel<ET, 8, 4, R>), grid, dim3(256), 0, s, p);
+  else if (V <= 64) RL_LAUNCH((loss_group_kernel<ET, 16, 4, R>), grid, dim3(256), 0, s, p);
+  else RL_LAUNCH((loss_group_kernel<ET, 16, 8, R>), grid, dim3(256), 0, s, p);
+}
+
 template <typename ET>
 int run(LossArgs p, const LossPlan& q, hipStream_t s) {
   typedef typename Elem<ET>::type E;
   const int V = p.V;
   const int64_t vecs = ceil_div((int64_t)V, (int64_t)Row16<E>::n);
   if (V <= kGroupV) {
-    const dim3 grid((unsigned)ceil_div(p.n_rows, 256 / group_lanes(V)));
-    if (V <= 8) RL_LAUNCH((loss_group_kernel<ET, 8, 1>), grid, dim3(256), 0, s, p);
-    else if (V <= 32) RL_LAUNCH((loss_group_kernel<ET, 8, 4>), grid, dim3(256), 0, s, p);
-    else if (V <= 64) RL_LAUNCH((loss_group_kernel<ET, 16, 4>), grid, dim3(256), 0, s, p);
-    else RL_LAUNCH((loss_group_kernel<ET, 32, 4>), grid, dim3(256), 0, s, p);
+    if (group_rows(p.N) == 1) launch_groups<ET, 1>(p, s);
+    else launch_groups<ET, 4>(p, s);
   } else if (V * (int64_t)sizeof(E) <= kWaveBytes) {
     const dim3 grid((unsigned)ceil_div(p.n_rows, 4));
     if (vecs <= 64) RL_LAUNCH((loss_wave_kernel<ET, 1>), grid, dim3(256), 0, s, p);

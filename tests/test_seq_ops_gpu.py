@@ -474,16 +474,16 @@ def test_policy_kl_loss_far_logits_and_ratios():
     assert abs(float(loss) + 1.3 * 0.5) < 1e-6 and not bool(grad.any())
 
 
-def test_policy_kl_loss_sums_over_many_rows(N=20000, V=200):
+def test_policy_kl_loss_sums_over_many_rows(N=20000, V=200, dtype=torch.float32):
     # more rows than one workgroup adds: shares first.  (Sums over rows are 64 bits, so the tolerances do not grow.)
-    data = loss_data(N, V, torch.float32, 52)
+    data = loss_data(N, V, dtype, 52)
     c = dict(kl_coeff=0.1, entropy_coeff=0.02)
     logits, action, old, adv, ref, w = data
     # a row's gradient is w / sum w times p or 1 - p times the sum of -r A, -0.1 (e^d - 1) and 0.02 (log p + H): with log p known
     # to err, r and e^d are to err relative; in some of many rows the three cancel to less than err of their sizes
     lp = torch.log_softmax(logits.double(), -1).gather(-1, action[:, None]).squeeze(-1)
     parts = (lp - old).exp() * adv.abs() + 0.1 * ((ref - lp).exp() + 1.) + 0.02 * math.log(V)
-    loss_close(*run_loss(*data, **KW, **c), *loss64(logits, action, old, adv, ref, w, 0.2, 0.3, 0.1, 0.02),
+    loss_close(*run_loss(*data, **KW, **c), *loss64(*data, 0.2, 0.3, 0.1, 0.02),
                cancel=(parts * w / w.double().sum())[:, None])
 
 

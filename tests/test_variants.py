@@ -852,10 +852,18 @@ def _policy_loss_case(dtype, N, V):
     return run
 
 
+def _policy_loss_many_case(dtype, N, V):
+    def run():
+        import test_seq_ops_gpu as P
+        P.test_policy_kl_loss_sums_over_many_rows(N, V, dtype)
+    return run
+
+
 for _e, _t in SEQ_TYPES.items():
     _n = 2 if _e == "float" else 4       # thousands of elements in 8 KB
-    for _k, _v in (("8, 1", 7), ("8, 4", 20), ("16, 4", 50), ("32, 4", 100)):
-        case(f"loss_group_kernel<{_e}, {_k}>")(_policy_loss_case(_t, 37, _v))
+    for _k, _v in (("8, 1", 7), ("8, 4", 20), ("16, 4", 50), ("16, 8", 100)):
+        case(f"loss_group_kernel<{_e}, {_k}, 1>")(_policy_loss_case(_t, 37, _v))
+        case(f"loss_group_kernel<{_e}, {_k}, 4>")(_policy_loss_many_case(_t, 32773, _v))
     for _k, _v in ((1, 100), (2, 200), (4, 500)):
         case(f"loss_wave_kernel<{_e}, {_k}>")(_policy_loss_case(_t, 37, _n * _v + 1))
     for _k, _v in (("256, 2", 750), ("256, 4", 1750), ("512, 4", 3500), ("1024, 4", 7500), ("1024, 8", 15000),
@@ -867,7 +875,7 @@ for _e, _t in SEQ_TYPES.items():
 @case("loss_finish_kernel", "loss_sum_kernel<float, 1>", "loss_sum_kernel<double, 1>", "loss_sum_kernel<double, 4>")
 def _policy_loss_sums():
     import test_seq_ops_gpu as P
-    P.test_policy_kl_loss_sums_over_many_rows(600000, 3)
+    P.test_policy_kl_loss_sums_over_many_rows(2200000, 3)
 
 
 def _policy_loss_scale_case(dtype):
