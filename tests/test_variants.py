@@ -864,9 +864,9 @@ for _e, _t in SEQ_TYPES.items():
     for _k, _v in (("8, 1", 7), ("8, 4", 20), ("16, 4", 50), ("16, 8", 100)):
         case(f"loss_group_kernel<{_e}, {_k}, 1>")(_policy_loss_case(_t, 37, _v))
         case(f"loss_group_kernel<{_e}, {_k}, 4>")(_policy_loss_many_case(_t, 32773, _v))
-    for _k, _v in ((1, 100), (2, 200), (4, 500)):
+    for _k, _v in ((1, 100), (2, 200), (4, 500), (8, 900)):
         case(f"loss_wave_kernel<{_e}, {_k}>")(_policy_loss_case(_t, 37, _n * _v + 1))
-    for _k, _v in (("256, 2", 750), ("256, 4", 1750), ("512, 4", 3500), ("1024, 4", 7500), ("1024, 8", 15000),
+    for _k, _v in (("256, 4", 1750), ("512, 4", 3500), ("1024, 4", 7500), ("1024, 8", 15000),
                    ("1024, 16", 30000)):
         case(f"loss_row_kernel<{_e}, {_k}>")(_policy_loss_case(_t, 256, _n * _v + 1))
     case(f"loss_parts_kernel<{_e}>", f"loss_join_kernel<{_e}>")(_policy_loss_case(_t, 3, 70001))
