@@ -154,6 +154,7 @@ __device__ __forceinline__ void segment_carry(const Args& p, const Lane& l, int 
 #pragma unroll
   for (int k = 0; k < V; ++k) A[k] = 1.f, H[k] = 0.f;
   if (l.on) {
+#pragma unroll 8
     for (int j = lo; j < hi; ++j) {
       const float2* q = p.agg + (int64_t)(FWD ? j : S - 1 - j) * C + l.c;
 #pragma unroll
