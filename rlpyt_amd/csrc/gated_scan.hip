@@ -13,6 +13,10 @@
 // launch reduces every segment to its map (it reads the streams without writing), the main launch folds the
 // maps of the segments before its own.  No workgroup ever waits for another one.
 //
+// Measured, against 4.64 TB/s of a large copy: 128 x 256 x 512 bf16 forward 25 us (103 MB, 4.1 TB/s), backward 38 us (170 MB,
+// 4.5); 65536 x 1 x 1024 bf16 in 64 segments 75 + 75 us forward, 62 + 150 backward, where one pass over the streams
+// would take 87 and 145; 85 x 32 x 512 f32 7.7 and 10.8 us, most of it latency (256 workgroups, two windows each).
+//
 // A reset forgets whatever came before, also a state that is not finite: such a map carries A = -1
 // (a product of sigmoids is never negative) and composes as "H alone", not as 0 * h.
 //

@@ -14,7 +14,12 @@
 // Storage of a factor with K columns (padded to the tile side, pads are 0): per row and 32 columns, 64 bytes of hi and 64 of lo.
 // All products are row-times-row ("A B^T"): X X^T takes X, A A takes A (symmetric), Q X takes Q and X^T, so an epilogue
 // writes its tile both ways.  Symmetric products compute the tiles on and above the diagonal and mirror them.
-// The matrices of a list go through each launch together: 2 + 3 steps launches for up to 32 of them.
+// The matrices of a list go through each launch together: up to 32 of them in 2 launches and 3 a step, and one more for a product
+// whose sums are split.
+//
+// Measured: 4096 x 4096, a symmetric product 206 us (1.0 PF/s of f16 operations, half of them counted), a full one 365 us (1.13);
+// a library's f16 product of 8192 reaches 1.2.  512 x 3456 with three small ones: 11 + 4 (X X^T, in four slices), 9 and 16 us a
+// step, of which 1.5 to 3 are matrix instructions; the rest is the way of the tiles from L2 and the launches' own latency.
 #include <limits.h>
 #include <math.h>
 

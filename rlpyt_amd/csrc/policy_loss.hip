@@ -11,6 +11,10 @@
 // and batches of so few rows that one workgroup each leaves the chip idle, are split over workgroups: one
 // launch for the statistics of the parts, one that joins them and reads the row again for the gradient.
 //
+// Measured, against 4.64 TB/s of a large copy: 8192 x 32000 bf16 (a fifth of the rows padded) 200 us, 226 being what a copy
+// of all its logits takes; 96 x 100003 f32, split, 11.5 + 16.5 us for a floor of 16.5; 8192 x 18 f32 6 us, and 4
+// each for the sums of the weights and over the rows.
+//
 // Sums over a row are f32 per lane and in a fixed order (no atomics); what is done once per row is in 64 bits, on f32
 // logarithms and exponentials of reduced arguments: kl ~ d^2 / 2 cancels in 32.  Exponents are in base 2 and come from one fma,
 // t = x log2(e) - m with m the rounded product of the largest logit; what that rounding took is put back per row.  Where m is
