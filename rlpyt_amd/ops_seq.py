@@ -10,6 +10,9 @@ the C ABI (``include/rlpyt_hip.h``); ``rlpyt_amd.ops`` offers them with the othe
 Arguments that do not fit raise ``ValueError`` before anything is launched.  Kernels run on the current stream of the
 tensors' device; workspaces come from torch's allocator per call, so that captured graphs do not share them.  Behind the
 checks, the first four run in a small extension (``csrc/seqops.cpp``): allocations, launches and autograd nodes.
+
+A backward pass that is captured into a graph needs what all of torch's autograd needs there: warm up on a side stream, and
+drop eager results that still hang on the same leaves (their nodes belong to the other stream).
 """
 import ctypes
 
