@@ -269,7 +269,7 @@ class Muon(torch.optim.Optimizer):
         bufs = [self.state[p]["momentum_buffer"] for p in params]
         torch._foreach_lerp_(bufs, grads, 1. - beta)
         updates = torch._foreach_lerp(grads, bufs, beta) if group["nesterov"] else bufs
-        updates = orthogonalize([u.reshape(u.shape[0], -1) for u in updates], steps=group["ns_steps"],
+        updates = orthogonalize([u.flatten(1) for u in updates], steps=group["ns_steps"],
                                 coeffs=group["ns_coeffs"], eps=group["ns_eps"])
         if group["weight_decay"]:
             torch._foreach_mul_(params, 1. - lr * group["weight_decay"])

@@ -853,6 +853,19 @@ def test_muon_of_16_bit_parameters_keeps_its_buffers_in_32():
     assert buf.dtype == torch.float32 and torch.equal(buf, opt.state[w]["momentum_buffer"])
 
 
+def test_muon_of_empty_and_missing_gradients():
+    from rlpyt_amd.optim import Muon
+    ps = [torch.zeros(3, 0, device=DEV, requires_grad=True), torch.ones(4, 5, device=DEV, requires_grad=True),
+          torch.ones(6, 2, device=DEV, requires_grad=True), torch.zeros(0, device=DEV, requires_grad=True)]
+    opt = Muon(ps)
+    opt.step()                               # no gradient at all
+    for p in (ps[0], ps[1], ps[3]):
+        p.grad = torch.ones_like(p)
+    norm = opt.clip_and_step(1.)
+    assert abs(float(norm) - math.sqrt(20)) < 1e-5
+    assert bool((ps[1] < 1).all()) and bool((ps[2] == 1).all()) and ps[0].shape == (3, 0)
+
+
 def test_a_recurrent_policy_trains_with_the_operators_together():
     """Embedding, gated recurrence over time with resets and padding, logits, loss, Muon: gradients of every
     parameter against the same network in 64 bits, an update, and the sampler's one-step form on the way."""
