@@ -4,12 +4,14 @@
 // Python's allocations and calls take twice as long.  Arguments are checked by rlpyt_amd/ops_seq.py.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <initializer_list>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -57,6 +59,24 @@ variable_list once(variable_list grads) {
   const variable_list out = (*node)(std::move(in));
   for (size_t i = 0; i < places.size(); ++i) grads[places[i]] = out[i];
   return grads;
+}
+
+// A captured backward pass would wait for the stream of the node that gathers a leaf's gradient.  Where an eager graph of the
+// leaf lives, that is the eager graph's, which a capture cannot wait for (the process ends): refused here.
+void check_leaves(const char* what, std::initializer_list<const Tensor*> inputs) {
+  const Tensor& first = **inputs.begin();
+  const c10::DeviceGuard guard(first.device());
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto current = c10::hip::getCurrentHIPStream(first.device().index());
+  for (const Tensor* t : inputs) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!node) continue;
+    const auto other = node->stream();
+    if (other && other->id() != current.id())
+      throw std::runtime_error(std::string(what) + ": a result computed from the same leaf on another stream is still held; "
+                               "drop it before its backward pass is captured");
+  }
 }
 
 // ---- gated linear recurrence ------------------------------------------------------------------------------
@@ -135,6 +155,8 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
 std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gate, const Maybe& h0, const Maybe& reset,
                                       const Maybe& lengths) {
   if (at::GradMode::is_enabled() && (x.requires_grad() || gate.requires_grad() || (h0 && h0->requires_grad()))) {
+    const Tensor state = or_none(h0);
+    check_leaves("gated_scan", {&x, &gate, &state});
     const variable_list out = GatedScan::apply(x, gate, h0, reset, lengths);
     return {out[0], out[1]};
   }
@@ -223,6 +245,7 @@ std::tuple<Tensor, Tensor> policy_kl_loss(const Tensor& logits, const Tensor& ro
                                           double grad_scale, int64_t unit_seed) {
   const Coeffs c = {low, high, kl, entropy, grad_scale};
   if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    check_leaves("policy_kl_loss", {&logits});
     const variable_list out =
         PolicyLoss::apply(logits, rows, action, old_logp, advantage, ref_logp, valid, c, unit_seed);
     return {out[0], out[1]};

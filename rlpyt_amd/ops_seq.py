@@ -12,7 +12,8 @@ tensors' device; workspaces come from torch's allocator per call, so that captur
 checks, the first four run in a small extension (``csrc/seqops.cpp``): allocations, launches and autograd nodes.
 
 A backward pass that is captured into a graph needs what all of torch's autograd needs there: warm up on a side stream, and
-drop eager results that still hang on the same leaves (their nodes belong to the other stream).
+drop eager results that still hang on the same leaves (their nodes belong to the other stream; an operator whose own
+input is such a leaf raises ``RuntimeError``).
 """
 import ctypes
 

@@ -752,6 +752,64 @@ def test_operators_replayed_in_a_graph_while_eager_work_runs():
             assert torch.equal(a, b)
 
 
+def test_backward_pass_captured_with_its_leaves():
+    """``loss.backward()`` into ``.grad`` within a graph: a projection, the scan, the loss."""
+    T, B, D, V = 40, 3, 32, 50
+    g = gen(105)
+    feed = torch.randn(T, B, D, device=DEV, generator=g)
+    w = (torch.randn(2 * D, D, device=DEV, generator=g) * 0.2).requires_grad_(True)
+    head = (torch.randn(V, D, device=DEV, generator=g) * 0.2).requires_grad_(True)
+    action = torch.randint(0, V, (T, B), device=DEV, generator=g)
+    old, adv = torch.full((T, B), -4., device=DEV), torch.randn(T, B, device=DEV, generator=g)
+
+    def work(w, head):
+        x, gate = torch.nn.functional.linear(feed, w).chunk(2, -1)
+        h, _ = ops.gated_scan(x, gate)
+        loss, scalars = ops.policy_kl_loss(torch.nn.functional.linear(h, head), action, old, adv, entropy_coeff=0.01)
+        loss.backward()
+        return scalars
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            work(w, head)
+    torch.cuda.current_stream().wait_stream(side)
+    w.grad = head.grad = None
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        scalars = work(w, head)
+    for k in range(4):
+        feed.mul_(1. + 0.1 * k)
+        graph.replay()
+        torch.cuda.synchronize()
+        other = [t.detach().clone().requires_grad_(True) for t in (w, head)]
+        want = work(*other)
+        assert torch.equal(scalars, want)
+        # (the library's products of an eager call may be other kernels than the captured ones': 2^-24 of up to 120 terms)
+        for a, b in zip((w, head), other):
+            assert torch.allclose(a.grad, b.grad, rtol=1e-4, atol=1e-6)
+
+
+def test_capture_is_refused_while_an_eager_graph_of_the_leaf_lives():
+    x, gate = (torch.randn(4, 2, 8, device=DEV, generator=gen(106)).requires_grad_(True) for _ in range(2))
+    logits = torch.randn(4, 9, device=DEV, generator=gen(107)).requires_grad_(True)
+    action, zero = torch.zeros(4, dtype=torch.long, device=DEV), torch.zeros(4, device=DEV)
+    calls = (lambda: ops.gated_scan(x, gate), lambda: ops.policy_kl_loss(logits, action, zero, zero))
+    for call in calls:
+        held = call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="drop it before"):
+            with torch.cuda.graph(graph):
+                call()
+        with torch.no_grad(), torch.cuda.graph(torch.cuda.CUDAGraph()):    # without a backward pass it may be captured
+            call()
+        del held
+        call()                               # and eager calls go on
+
+
 def test_operators_on_two_streams_at_once():
     streams = [torch.cuda.Stream() for _ in range(2)]
     datas = [scan_data(3000, 1, 130, torch.bfloat16, 110 + k, True) for k in range(2)]
