@@ -47,8 +47,10 @@ struct Mat {
   int rows, cols;
   int mp, np;                        // padded sides of X: min and max
   int tall;
-  _Float16 *x, *xt[2], *a, *q;       // X [mp, np], X^T [np, mp] (two: read and written), A, Q [mp, mp]
+  _Float16 *x, *xt0, *xt1, *a, *q;   // X [mp, np], X^T [np, mp] (two: read and written), A, Q [mp, mp]
   double* norm;                      // [kNormBlocks]
+  // (an array here puts a kernel's copy of this struct into scratch memory: 128 x 128 took 84 us instead of 75)
+  __device__ _Float16* xt(int k) const { return k ? xt1 : xt0; }
 };
 // The first launch gets the table as its argument and leaves it in the workspace for the others: an argument is read from the
 // host's memory, 3 KB of it by every launch.
@@ -147,7 +149,7 @@ __global__ __launch_bounds__(256) void ns_load_kernel(const Mats* __restrict__ t
     _Float16* p = M.x + at(r0 + k, c0 + lx, M.np);
     p[0] = hi, p[32] = lo;
     split(tile[lx][k], hi, lo);
-    p = M.xt[0] + at(c0 + k, r0 + lx, M.mp);
+    p = M.xt0 + at(c0 + k, r0 + lx, M.mp);
     p[0] = hi, p[32] = lo;
   }
 }
@@ -229,7 +231,7 @@ __device__ __forceinline__ void write_block(const Mat& M, int cur, const Coeffs&
       o[0] = vh, o[32] = vl;
     }
     if (MODE == LAST || !both) continue;
-    _Float16* o = (MODE == GRAM ? M.a : MODE == POLY ? M.q : M.xt[cur ^ 1]) + at(col, row, M.mp);   // 4 consecutive columns
+    _Float16* o = (MODE == GRAM ? M.a : MODE == POLY ? M.q : M.xt(cur ^ 1)) + at(col, row, M.mp);   // 4 consecutive columns
     *(f16x4*)o = hi;
     *(f16x4*)(o + 32) = lo;
   }
@@ -274,7 +276,7 @@ __device__ __forceinline__ void write8(const Mat& M, int cur, const Coeffs& f, c
     split(v, vh, vl);
     hi[i] = vh, lo[i] = vl;
   }
-  _Float16* o = (MODE == GRAM ? M.a : MODE == POLY ? M.q : ROW ? M.x : M.xt[cur ^ 1]) + at(r, k, K);
+  _Float16* o = (MODE == GRAM ? M.a : MODE == POLY ? M.q : ROW ? M.x : M.xt(cur ^ 1)) + at(r, k, K);
   *(f16x8*)o = hi;
   *(f16x8*)(o + 32) = lo;
 }
@@ -331,7 +333,7 @@ __global__ __launch_bounds__((Shape<T, G_>::threads)) void ns_product_kernel(con
   const int tr = at_.tr, tc = at_.tc;
   const int K = MODE == GRAM ? M.np : M.mp;
   const _Float16* P = MODE == GRAM ? M.x : MODE == POLY ? M.a : M.q;
-  const _Float16* Q = MODE == GRAM ? M.x : MODE == POLY ? M.a : M.xt[cur];
+  const _Float16* Q = MODE == GRAM ? M.x : MODE == POLY ? M.a : M.xt(cur);
   const int lane = threadIdx.x & 63;
   const int set = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / G::waves;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - set * G::waves;
@@ -748,8 +750,8 @@ extern "C" int rlpyt_orthogonalize(int dtype, const void* const* in_host, const 
       m.in = in_host[l.place[i]], m.out = out_host[l.place[i]], m.ld = ld_host[l.place[i]];
       const int64_t big = (int64_t)m.mp * m.np * 2, small = (int64_t)m.mp * m.mp * 2;   // halves
       m.x = (_Float16*)ws;
-      m.xt[0] = m.x + big, m.xt[1] = m.xt[0] + big;
-      m.a = m.xt[1] + big, m.q = m.a + small;
+      m.xt0 = m.x + big, m.xt1 = m.xt0 + big;
+      m.a = m.xt1 + big, m.q = m.a + small;
       m.norm = (double*)(m.q + small);
       ws += factor_bytes(m);
     }
