@@ -11,6 +11,9 @@ Arguments that do not fit raise ``ValueError`` before anything is launched.  Ker
 tensors' device; workspaces come from torch's allocator per call, so that captured graphs do not share them.  Behind the
 checks, the first four run in a small extension (``csrc/seqops.cpp``): allocations, launches and autograd nodes.
 
+Small calls wait for autograd's device thread longer than for the device: a program with one GPU may run its backward passes
+under ``torch.autograd.set_multithreading_enabled(False)``, which halves a small scan's time.
+
 A backward pass that is captured into a graph needs what all of torch's autograd needs there: warm up on a side stream, and
 drop eager results that still hang on the same leaves (their nodes belong to the other stream; an operator whose own
 input is such a leaf raises ``RuntimeError``).
