@@ -12,8 +12,8 @@
 // launch for the statistics of the parts, one that joins them and reads the row again for the gradient.
 //
 // Measured, against 4.64 TB/s of a large copy: 8192 x 32000 bf16 (a fifth of the rows padded) 200 us, 226 being what a copy
-// of all its logits takes; 96 x 100003 f32, split, 11.5 + 16.5 us for a floor of 16.5; 8192 x 18 f32 6 us, and 4
-// each for the sums of the weights and over the rows.
+// of all its logits takes; 96 x 100003 f32, split, 11.5 + 16.5 us for a floor of 16.5; 8192 x 18 f32 8 us with the
+// sum of the weights, and 4 for the sums over the rows.
 //
 // Sums over a row are f32 per lane and in a fixed order (no atomics); what is done once per row is in 64 bits, on f32
 // logarithms and exponentials of reduced arguments: kl ~ d^2 / 2 cancels in 32.  Exponents are in base 2 and come from one fma,
@@ -44,7 +44,7 @@ struct LossArgs {
   void* grad;                     // [N, V] dense, or null
   float *logp, *entropy;          // [N] each, or null
   double* rows;                   // [n, 4]: w pi, w kl, w H, w clipped of a row (or workgroup), or null (log-probabilities only)
-  const double* denom;            // sum of valid, or null: N
+  const double* denom;            // sum of valid, or null: N, or summed by every workgroup for itself
   struct Stats* parts;            // split rows: statistics of the parts [N, P]
   int64_t N, n0, n_rows;          // a launch takes the rows n0 .. n0 + n_rows - 1
   int V, part;                    // part: elements of a row's part, a multiple of 8
@@ -107,6 +107,21 @@ __device__ __forceinline__ double kl_of(double d) {
   return 0.5 * d * d * v;
 }
 
+// What the mean divides by; every thread of the workgroup has to come here.
+__device__ __forceinline__ double weights(const float* __restrict__ valid, int64_t N, const double* denom, double* scratch) {
+  if (!valid) return (double)N;
+  if (denom) return *denom;
+  double v = 0.0;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < N; i += blockDim.x) v += (double)valid[i];
+  v = wave_sum(v);
+  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.0;
+  for (int i = 0; i < (int)(blockDim.x >> 6); ++i) v += scratch[i];
+  return v;
+}
+
 // What follows from a row's statistics: its terms of the loss, and its gradient as 2^t (k1 t + k0), + ka at the action, with
 // t = (x - base) log2(e) - m, of which one is 0.
 struct RowOut {
@@ -114,7 +129,7 @@ struct RowOut {
   float logp, entropy, base, m, k1, k0, ka;
 };
 __device__ __forceinline__ RowOut row_terms(const LossArgs& p, int64_t n, float w, const Stats& st, float xa,
-                                            bool in_range) {
+                                            bool in_range, double denom) {
   RowOut o = {};
   if (st.m == -INFINITY && st.s == 0.f) {   // every logit is -inf: no distribution, the row adds nothing and has no gradient
     o.logp = -INFINITY;
@@ -145,7 +160,6 @@ __device__ __forceinline__ RowOut row_terms(const LossArgs& p, int64_t n, float 
     c -= p.c_kl * (o.kl + d);
   }
   o.ent = H;
-  const double denom = p.denom ? *p.denom : (double)p.N;
   const double g = denom > 0.0 ? p.g_scale * (double)w / denom : 0.0, gs = g / (double)st.s;
   o.k1 = (float)(gs * p.c_ent * kLn2);
   o.k0 = (float)(gs * (p.c_ent * (H - logs) - c));
@@ -174,7 +188,7 @@ template <typename ET, int G, int K, int R>
 __global__ __launch_bounds__(256) void loss_group_kernel(const LossArgs p) {
   typedef typename Elem<ET>::type E;
   constexpr int each = 256 / G;           // groups of a workgroup, and rows of a round
-  __shared__ double sums[4 * 16];
+  __shared__ double sums[4 * 16], ws[4];
   const int sub = threadIdx.x & (G - 1);
   const int64_t first = p.n0 + (int64_t)blockIdx.x * (each * R) + threadIdx.x / G, end = p.n0 + p.n_rows;
   const int64_t own = first + sub * each;    // the row whose terms this lane works out
@@ -194,6 +208,7 @@ __global__ __launch_bounds__(256) void loss_group_kernel(const LossArgs p) {
       t[r][k] = live && j < p.V ? (float)row[j] : -INFINITY;
     }
   }
+  const double denom = weights(p.valid, p.N, p.denom, ws);
   Stats st = {-INFINITY, 0.f, 0.f};
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -215,7 +230,7 @@ __global__ __launch_bounds__(256) void loss_group_kernel(const LossArgs p) {
   }
   RowOut o = {};
   if (w != 0.f) {
-    o = row_terms(p, own, w, st, xa, in_range);
+    o = row_terms(p, own, w, st, xa, in_range, denom);
     if (p.logp) p.logp[own] = o.logp, p.entropy[own] = o.entropy;
   }
   if (p.grad) {
@@ -357,6 +372,7 @@ __global__ __launch_bounds__(NT) void loss_row_kernel(const LossArgs p) {
   constexpr int n16 = Row16<E>::n;
   __shared__ Stats lds[NT / kWave];
   __shared__ RowOut out;
+  __shared__ double ws[NT / kWave];
   const int64_t n = p.n0 + blockIdx.x;
   const float w = p.valid ? p.valid[n] : 1.f;
   E* g = p.grad ? (E*)p.grad + n * p.V : nullptr;
@@ -380,10 +396,11 @@ __global__ __launch_bounds__(NT) void loss_row_kernel(const LossArgs p) {
   vec x[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) x[r] = load16<E>(row, (r * NT + threadIdx.x) * n16, p.V);
+  const double denom = weights(p.valid, p.N, p.denom, ws);
   const Stats st = block_join<NT>(wave_stats<E, R>(x), lds);
   forget<E, R>(x);
   if (threadIdx.x == 0) {
-    out = row_terms(p, n, w, st, xa, in_range);
+    out = row_terms(p, n, w, st, xa, in_range, denom);
     if (p.logp) p.logp[n] = out.logp, p.entropy[n] = out.entropy;
     if (p.rows) p.rows[n * 4] = out.pi, p.rows[n * 4 + 1] = out.kl, p.rows[n * 4 + 2] = out.ent, p.rows[n * 4 + 3] = out.clipped;
   }
@@ -404,11 +421,12 @@ __global__ __launch_bounds__(256) void loss_wave_kernel(const LossArgs p) {
   typedef typename Elem<ET>::type E;
   typedef typename Row16<E>::vec vec;
   constexpr int n16 = Row16<E>::n;
-  __shared__ double sums[4][4];
+  __shared__ double sums[4][4], ws[4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t n = p.n0 + (int64_t)blockIdx.x * 4 + wave;
   const bool on = n < p.n0 + p.n_rows;
   const float w = on ? (p.valid ? p.valid[n] : 1.f) : 0.f;
+  const double denom = weights(p.valid, p.N, p.denom, ws);
   RowOut o = {};
   if (w != 0.f) {
     const E* row = (const E*)p.logits + n * p.row_stride;
@@ -418,7 +436,7 @@ __global__ __launch_bounds__(256) void loss_wave_kernel(const LossArgs p) {
     vec x[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) x[r] = load16<E>(row, (r * kWave + lane) * n16, p.V);
-    o = row_terms(p, n, w, wave_stats<E, R>(x), xa, in_range);
+    o = row_terms(p, n, w, wave_stats<E, R>(x), xa, in_range, denom);
     forget<E, R>(x);
     if (lane == 0 && p.logp) p.logp[n] = o.logp, p.entropy[n] = o.entropy;
     if (p.grad) {
@@ -477,6 +495,7 @@ __global__ __launch_bounds__(kSplitThreads) void loss_join_kernel(const LossArgs
   constexpr int n16 = Row16<E>::n, step = kSplitThreads * n16;
   __shared__ Stats lds[kSplitThreads / kWave];
   __shared__ RowOut out;
+  __shared__ double ws[kSplitThreads / kWave];
   const int64_t n = p.n0 + blockIdx.x / blocks;   // blocks per row: P, or 1 without a gradient
   const int part = blockIdx.x % blocks;
   const float w = p.valid ? p.valid[n] : 1.f;
@@ -487,10 +506,11 @@ __global__ __launch_bounds__(kSplitThreads) void loss_join_kernel(const LossArgs
   if (live) {
     Stats st = {-INFINITY, 0.f, 0.f};
     for (int i = threadIdx.x; i < P; i += kSplitThreads) st = join(st, p.parts[n * P + i]);
+    const double denom = weights(p.valid, p.N, p.denom, ws);
     st = block_join<kSplitThreads>(group_join<kWave>(st), lds);
     if (threadIdx.x == 0) {
       const bool in_range = a >= 0 && a < p.V;
-      out = row_terms(p, n, w, st, in_range ? (float)row[a] : 0.f, in_range);
+      out = row_terms(p, n, w, st, in_range ? (float)row[a] : 0.f, in_range, denom);
       if (first && p.logp) p.logp[n] = out.logp, p.entropy[n] = out.entropy;
     }
   } else if (threadIdx.x == 0) {
@@ -535,10 +555,12 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const T* __restrict__ in
 }
 
 __global__ __launch_bounds__(1024) void loss_finish_kernel(const double* __restrict__ rows, int64_t n,
-                                                           const double* __restrict__ denom, double N, double c_kl,
+                                                           const double* __restrict__ denom,
+                                                           const float* __restrict__ valid, int64_t N, double c_kl,
                                                            double c_ent, float* __restrict__ loss,
                                                            float* __restrict__ scalars) {
-  __shared__ double scratch[4 * 16];
+  __shared__ double scratch[4 * 16], ws[16];
+  const double d = weights(valid, N, denom, ws);
   double v[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll 4
   for (int64_t i = threadIdx.x; i < n; i += 1024)
@@ -546,7 +568,6 @@ __global__ __launch_bounds__(1024) void loss_finish_kernel(const double* __restr
     for (int k = 0; k < 4; ++k) v[k] += rows[i * 4 + k];
   block_sum<4>(v, scratch);
   if (threadIdx.x != 0) return;
-  const double d = denom ? *denom : N;
   const double inv = d > 0.0 ? 1.0 / d : 0.0;   // nothing valid: a loss of 0
   for (int k = 0; k < 4; ++k) v[k] *= inv;
   *loss = scalars[0] = (float)(v[0] + c_kl * v[1] - c_ent * v[2]);
@@ -585,6 +606,7 @@ constexpr int kWaveBytes = 8192;
 struct LossPlan {
   int P, part;                      // P > 0: rows split into P parts of `part` elements
   int64_t partials;                 // rows of the [., 4] table of partial sums
+  int64_t groups(int64_t N) const { return P > 0 ? N * P : partials; }   // workgroups
 };
 int group_lanes(int64_t V) { return V <= 32 ? 8 : 16; }
 // Rows of a group.  262144 x 18 in f32 takes 49 us by one row each and 35 by four, 8192 x 18 18.4 and 19.1 (fewer
@@ -706,14 +728,17 @@ extern "C" int rlpyt_policy_kl_loss_fwd_bwd(int dtype, const void* logits, int64
   p.ref_logp = ref_logp, p.valid = valid, p.grad = grad;
   double *denom = (double*)workspace, *shares = (double*)((char*)workspace + 16);
   p.rows = (double*)((char*)workspace + kRowsOffset);
-  p.denom = valid ? denom : nullptr;
+  // The sum of the weights: by every workgroup where that is few numbers altogether, else in a launch of its own.  (8192 x 18: 17 us
+  // on the device either way, and 4 us less of the call.)
+  const bool fold = q.groups(N) * N <= (int64_t)1 << 21;
+  p.denom = valid && !fold ? denom : nullptr;
   p.parts = (Stats*)((char*)workspace + parts_offset(q));
   p.N = N, p.V = (int)V, p.part = q.part;
   p.lo = clip_low, p.hi = clip_high, p.c_kl = kl_coeff, p.c_ent = entropy_coeff, p.g_scale = grad_scale;
-  if (valid && N > kSumRows) {
+  if (p.denom && N > kSumRows) {
     RL_LAUNCH((loss_sum_kernel<float, 1>), dim3(kSumBlocks), dim3(1024), 0, s, valid, N, shares);
     RL_LAUNCH((loss_sum_kernel<double, 1>), dim3(1), dim3(1024), 0, s, shares, kSumBlocks, denom);
-  } else if (valid) {
+  } else if (p.denom) {
     RL_LAUNCH((loss_sum_kernel<float, 1>), dim3(1), dim3(1024), 0, s, valid, N, denom);
   }
   const int rc = run_all(dtype, p, q, s);
@@ -724,8 +749,8 @@ extern "C" int rlpyt_policy_kl_loss_fwd_bwd(int dtype, const void* logits, int64
     RL_LAUNCH((loss_sum_kernel<double, 4>), dim3(kSumBlocks), dim3(1024), 0, s, rows, sums, shares);
     rows = shares, sums = kSumBlocks;
   }
-  RL_LAUNCH(loss_finish_kernel, dim3(1), dim3(1024), 0, s, rows, sums, p.denom, (double)N, kl_coeff, entropy_coeff, loss,
-            scalars);
+  RL_LAUNCH(loss_finish_kernel, dim3(1), dim3(1024), 0, s, rows, sums, p.denom, valid, N, kl_coeff,
+            entropy_coeff, loss, scalars);
   RL_LAUNCH_CHECK();
   return RLPYT_OK;
 }

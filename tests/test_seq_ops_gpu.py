@@ -487,6 +487,10 @@ def test_policy_kl_loss_sums_over_many_rows(N=20000, V=200, dtype=torch.float32)
                cancel=(parts * w / w.double().sum())[:, None])
 
 
+def test_policy_kl_loss_weights_summed_in_a_launch_of_their_own():
+    test_policy_kl_loss_sums_over_many_rows(4000, 200)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("V", [5, 30, 100, 900, 3500, 40000])
 def test_policy_kl_loss_of_huge_logits(V, dtype):
