@@ -1,6 +1,9 @@
 """Refusals of the sequence operators (no GPU needed): wrong shapes, types and options raise before any device
 call, and the C entry points return error codes with a message."""
 import ctypes
+import os
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -117,3 +120,38 @@ def test_entry_points_validate_without_a_gpu():
     assert orth(0, one, side, one, side, side, 1, 5, 9., 0., 0., 0., p, None) != 0     # leaves f16's range
     assert b"range of the stored factors" in lib.rlpyt_hip_last_error()
     assert orth(0, one, side, one, side, side, 1, 5, float("nan"), 0., 0., 0., p, None) != 0
+
+
+LOSS_PLAN = r"""
+#include <cstdint>
+#include <cstdio>
+namespace rlpyt { static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; } }
+#include "policy_loss_plan.h"
+int main() {
+  using namespace rlpyt;
+  int bad = 0;
+  for (int size : {2, 4})
+    for (int64_t V : {1, 5, 128, 129, 4096, 4097, 32768, 32769, 65536, 65537, 131072, 131073, 300007, 1 << 30})
+      for (int64_t N : {0, 1, 3, 127, 128, 1023, 1025, 32768, 3000000}) {
+        const LossPlan q = plan_of(N, V, size);
+        const int64_t slice = slice_rows(q);
+        // parts that cover a row, none of them empty or off a 16-byte step; a launch of less than 2^32 threads
+        bool ok = q.P >= 0 && slice > 0 && slice * (q.P > 0 ? q.P * 256 : 1024) < (int64_t)1 << 32;
+        if (q.P > 0) ok = ok && q.part % 8 == 0 && (int64_t)q.part * q.P >= V && (int64_t)q.part * (q.P - 1) < V;
+        if (N == 0) ok = ok && q.groups(0) == 0;
+        if (!ok) ++bad, printf("N %ld V %ld size %d: P %d part %d\n", (long)N, (long)V, size, q.P, q.part);
+      }
+  return bad != 0;
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="no host compiler")
+def test_plan_of_the_policy_loss(tmp_path):
+    """Compiled on its own and unoptimised: an optimiser may drop a division by zero, the machine does not."""
+    src, exe = tmp_path / "plan.cpp", tmp_path / "plan"
+    src.write_text(LOSS_PLAN)
+    csrc = os.path.join(os.path.dirname(_lib.__file__), "csrc")
+    subprocess.run(["g++", "-std=c++17", "-O0", "-I", csrc, str(src), "-o", str(exe)], check=True)
+    run = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert run.returncode == 0, (run.returncode, run.stdout)

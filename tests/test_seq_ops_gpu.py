@@ -1003,3 +1003,19 @@ def test_ppo_takes_muon_as_its_optimizer():
     assert float(norm) > 1. and norm is out
     assert float(torch.nn.utils.get_total_norm([p.grad for p in params])) < 1.01 if hasattr(torch.nn.utils, "get_total_norm") else True
     assert isinstance(algo.clip_and_step(), torch.Tensor)
+
+
+@pytest.mark.parametrize("V", [5, 500, 20000, 40000, 70000])
+def test_policy_kl_loss_of_an_empty_batch(V):
+    """Rows of every plan: by groups, waves, workgroups and split (past 128 KB and past 256 KB in float32)."""
+    logits = torch.zeros(0, V, device=DEV, requires_grad=True)
+    none = torch.zeros(0, device=DEV)
+    for valid in (None, none):
+        loss, scalars = ops.policy_kl_loss(logits, none.long(), none, none, valid=valid, entropy_coeff=0.01)
+        grad, = torch.autograd.grad(loss, logits)
+        assert float(loss.detach()) == 0. and not bool(scalars.any()) and grad.shape == (0, V)
+        with torch.no_grad():
+            loss, scalars = ops.policy_kl_loss(logits, none.long(), none, none, valid=valid)
+        assert float(loss) == 0. and not bool(scalars.any())
+    lp, ent = ops.action_logp(logits.detach(), none.long())
+    assert lp.shape == (0,) and ent.shape == (0,)
