@@ -7,7 +7,8 @@ the C ABI (``include/rlpyt_hip.h``); ``rlpyt_amd.ops`` offers them with the othe
   ``ppo_loss``, which takes probabilities of a few actions;
 * ``orthogonalize``: the Newton-Schulz products behind ``rlpyt_amd.optim.Muon``.
 
-Arguments that do not fit raise ``ValueError`` before anything is launched.  Kernels run on the current stream of the
+Arguments that do not fit raise ``ValueError`` before anything is launched, tensors with a forward-mode derivative
+(``torch.autograd.forward_ad``) among them.  Kernels run on the current stream of the
 tensors' device; workspaces come from torch's allocator per call, so that captured graphs do not share them.  Behind the
 checks, the first four run in a small extension (``csrc/seqops.cpp``): allocations, launches and autograd nodes.
 
@@ -21,6 +22,7 @@ input is such a leaf raises ``RuntimeError``).
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, lib
@@ -52,6 +54,15 @@ def _need_device(name, first, *others):
     for t in others:
         if t is not None and t.device != device:
             _refuse(f"{name}: tensors on one device are needed, got {device} and {t.device}")
+
+
+def _no_tangents(name, *tensors):
+    """The kernels see values only: a forward-mode derivative would be lost without a word.  (Tangents live within a level.)"""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            _refuse(f"{name}: forward-mode derivatives are not supported")
 
 
 # --------------------------------------------------------------------------------------
@@ -93,6 +104,7 @@ def gated_scan(x, gate, h0=None, reset=None, lengths=None):
         _refuse(f"gated_scan: reset has to be [T, B], got {tuple(reset.shape)}")
     if lengths is not None and (lengths.shape != (B,) or lengths.dtype not in (torch.int32, torch.int64)):
         _refuse(f"gated_scan: lengths has to be [B], int32 or int64, got {tuple(lengths.shape)} {lengths.dtype}")
+    _no_tangents("gated_scan", x, gate, h0)
     _need_device("gated_scan", x, gate, h0, reset, lengths)
     if x.numel() == 0:
         hn = torch.zeros((B, D), dtype=torch.float32, device=x.device) if h0 is None else h0.float()
@@ -127,6 +139,7 @@ def gated_scan_step(x, gate, state, reset=None):
         _refuse(f"gated_scan_step: reset has to be [B], got {tuple(reset.shape)}")
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad):
         _refuse("gated_scan_step: not differentiable; call gated_scan, or this under torch.no_grad()")
+    _no_tangents("gated_scan_step", x, gate, state)
     _need_device("gated_scan_step", x, gate, state, reset)
     if reset is not None and not (reset.dtype in _BYTES and reset.is_contiguous()):
         reset = _reset_bytes(reset)
@@ -149,6 +162,7 @@ def _logit_rows(name, logits, action):
                 f"{logits.dtype}")
     if action.shape != logits.shape[:-1] or action.is_floating_point() or action.dtype == torch.bool:
         _refuse(f"{name}: one whole action per row of logits is needed, got {tuple(action.shape)} {action.dtype}")
+    _no_tangents(name, logits)
     _need_device(name, logits, action)
     rows = logits.detach()
     if rows.dim() != 2:
@@ -203,6 +217,7 @@ def policy_kl_loss(logits, action, old_logp, advantage, ref_logp=None, valid=Non
         _refuse("policy_kl_loss: kl_coeff needs ref_logp")
     if not 0. < grad_scale < float("inf"):
         _refuse("policy_kl_loss: a positive grad_scale is needed")
+    _no_tangents("policy_kl_loss", old_logp, advantage, ref_logp, valid)
     rows, action = _logit_rows("policy_kl_loss", logits, action)
     _need_device("policy_kl_loss", rows, old_logp, advantage, ref_logp, valid)
     seed = _unit_seeds.get(logits.device)
@@ -249,6 +264,7 @@ def orthogonalize(mats, steps=5, coeffs=NS_COEFFS, eps=1e-7):
             _refuse(f"orthogonalize: sides up to 65536 are supported, got {tuple(g.shape)}")
     if not mats:
         return []
+    _no_tangents("orthogonalize", *mats)
     _need_device("orthogonalize", *mats)
     device = mats[0].device
     outs, tables = [], {}

@@ -155,3 +155,33 @@ def test_plan_of_the_policy_loss(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-O0", "-I", csrc, str(src), "-o", str(exe)], check=True)
     run = subprocess.run([str(exe)], capture_output=True, text=True)
     assert run.returncode == 0, (run.returncode, run.stdout)
+
+
+@pytest.mark.parametrize("needs_grad", [False, True])
+def test_forward_mode_derivatives_are_refused(needs_grad):
+    """A dual tensor does not require a gradient by itself; its derivative must not get lost."""
+    fw = torch.autograd.forward_ad
+    with fw.dual_level():
+        def dual(*shape):
+            return fw.make_dual(z(*shape, requires_grad=needs_grad), torch.ones(*shape))
+
+        seq, row, one = z(3, 2, 4), z(2, 4), z(3)
+        calls = [
+            lambda: ops.gated_scan(dual(3, 2, 4), seq), lambda: ops.gated_scan(seq, dual(3, 2, 4)),
+            lambda: ops.gated_scan(seq, seq, h0=dual(2, 4)),
+            lambda: ops.policy_kl_loss(dual(3, 4), one.long(), one, one),
+            lambda: ops.policy_kl_loss(z(3, 4), one.long(), dual(3), one),
+            lambda: ops.policy_kl_loss(z(3, 4), one.long(), one, dual(3)),
+            lambda: ops.policy_kl_loss(z(3, 4), one.long(), one, one, ref_logp=dual(3)),
+            lambda: ops.policy_kl_loss(z(3, 4), one.long(), one, one, valid=dual(3)),
+            lambda: ops.action_logp(dual(3, 4), one.long()),
+            lambda: ops.orthogonalize(dual(4, 4)), lambda: ops.orthogonalize([z(4, 4), dual(2, 4, 4)]),
+        ]
+        steps = [lambda: ops.gated_scan_step(dual(2, 4), row, row), lambda: ops.gated_scan_step(row, dual(2, 4), row),
+                 lambda: ops.gated_scan_step(row, row, dual(2, 4))]
+        for call in calls:
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        for call in steps:
+            with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):     # (this mode goes on under no_grad)
+                call()
