@@ -162,7 +162,6 @@ def _logit_rows(name, logits, action):
                 f"{logits.dtype}")
     if action.shape != logits.shape[:-1] or action.is_floating_point() or action.dtype == torch.bool:
         _refuse(f"{name}: one whole action per row of logits is needed, got {tuple(action.shape)} {action.dtype}")
-    _no_tangents(name, logits)
     _need_device(name, logits, action)
     rows = logits.detach()
     if rows.dim() != 2:
@@ -217,7 +216,7 @@ def policy_kl_loss(logits, action, old_logp, advantage, ref_logp=None, valid=Non
         _refuse("policy_kl_loss: kl_coeff needs ref_logp")
     if not 0. < grad_scale < float("inf"):
         _refuse("policy_kl_loss: a positive grad_scale is needed")
-    _no_tangents("policy_kl_loss", old_logp, advantage, ref_logp, valid)
+    _no_tangents("policy_kl_loss", logits, old_logp, advantage, ref_logp, valid)
     rows, action = _logit_rows("policy_kl_loss", logits, action)
     _need_device("policy_kl_loss", rows, old_logp, advantage, ref_logp, valid)
     seed = _unit_seeds.get(logits.device)
@@ -228,8 +227,12 @@ def policy_kl_loss(logits, action, old_logp, advantage, ref_logp=None, valid=Non
 
 def action_logp(logits, action):
     """``(log softmax(logits)[action], entropy)``, float32, of every row of ``logits [..., V]`` (float32,
-    bfloat16 or float16): what ``policy_kl_loss`` takes as ``old_logp`` and ``ref_logp``.  Reads the logits once; not
-    differentiable.  A row of -inf only gives ``(-inf, 0)``, an action outside 0 .. V-1 NaN."""
+    bfloat16 or float16): what ``policy_kl_loss`` takes as ``old_logp`` and ``ref_logp``.  Reads the logits once.
+    A row of -inf only gives ``(-inf, 0)``, an action outside 0 .. V-1 NaN.  Not differentiable: logits that require a
+    gradient are taken under ``torch.no_grad()`` only."""
+    _no_tangents("action_logp", logits)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        _refuse("action_logp: not differentiable; call it under torch.no_grad() or with logits.detach()")
     rows, action = _logit_rows("action_logp", logits, action)
     return _seqops.action_logp(logits, rows, action)
 
@@ -248,7 +251,8 @@ def orthogonalize(mats, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     ``mats``: a tensor ``[..., m, n]`` or a list of such, float32, bfloat16 or float16; returned are new
     dense tensors of the same shapes and types.  All matrices of one type go through the same few launches.  Products
     have 22 bits and float32 sums whatever the type.  Entries below ``2^-37 |G|_F`` are lost, a zero matrix stays zero.
-    ``coeffs`` have to keep singular values of 0 .. 1 bounded (below sqrt(8) on the way).  Not differentiable."""
+    ``coeffs`` have to keep singular values of 0 .. 1 bounded (below sqrt(8) on the way).  Not differentiable: matrices that
+    require a gradient are taken under ``torch.no_grad()`` only."""
     single = isinstance(mats, torch.Tensor)
     mats = [mats] if single else list(mats)
     if int(steps) != steps or not 1 <= steps <= 100:
@@ -265,6 +269,8 @@ def orthogonalize(mats, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     if not mats:
         return []
     _no_tangents("orthogonalize", *mats)
+    if torch.is_grad_enabled() and any(g.requires_grad for g in mats):
+        _refuse("orthogonalize: not differentiable; call it under torch.no_grad() or with detached matrices")
     _need_device("orthogonalize", *mats)
     device = mats[0].device
     outs, tables = [], {}

@@ -185,3 +185,13 @@ def test_forward_mode_derivatives_are_refused(needs_grad):
         for call in steps:
             with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):     # (this mode goes on under no_grad)
                 call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda t: ops.action_logp(t, z(4).long()), lambda t: ops.orthogonalize(t), lambda t: ops.orthogonalize([z(3, 3), t]),
+])
+def test_gradients_that_would_be_lost_are_refused(call):
+    with pytest.raises(ValueError, match="not differentiable"):
+        call(z(4, 4, requires_grad=True))
+    with torch.no_grad(), pytest.raises((ValueError, _lib.HipError), match="device|MI355X"):     # (these are on the CPU)
+        call(z(4, 4, requires_grad=True))
