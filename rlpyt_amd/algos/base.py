@@ -6,6 +6,8 @@ attributes the runner reads).  On top of it this base owns the two things that d
 algorithm here: sample batches arrive as HBM tensors (anything that is not already on the agent's
 device is moved once, asynchronously) and diagnostics leave the device once per call instead of
 once per minibatch."""
+import inspect
+
 import torch
 
 
@@ -37,6 +39,13 @@ class RlAlgorithm:
         self.optimizer.load_state_dict(state_dict)
 
     # ------------------------------------------------------------------ optimizer
+    @staticmethod
+    def default_eps(OptimCls, eps):
+        """``dict(eps=eps)``, the DQN family's default for Adam, where the constructor of ``OptimCls`` takes one (RMSprop's does;
+        SGD's and Muon's do not)."""
+        takes = inspect.signature(OptimCls).parameters.values()
+        return dict(eps=eps) if any(p.name == "eps" or p.kind is p.VAR_KEYWORD for p in takes) else {}
+
     def make_optimizer(self, params, OptimCls, lr, optim_kwargs=None):
         """``OptimCls(params, lr=lr, **optim_kwargs)`` as the reference builds it
         (rlpyt/algos/pg/base.py:34-37, dqn/dqn.py:108-112) -- except that plain

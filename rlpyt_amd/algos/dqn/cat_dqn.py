@@ -15,8 +15,8 @@ class CategoricalDQN(DQN):
         super().__init__(**kwargs)
         self.V_min = V_min
         self.V_max = V_max
-        if "eps" not in self.optim_kwargs:  # assume Adam (cat_dqn.py:22-23)
-            self.optim_kwargs["eps"] = 0.01 / self.batch_size
+        # (also where other keywords were given: cat_dqn.py:22-23)
+        self.optim_kwargs = {**self.default_eps(self.OptimCls, 0.01 / self.batch_size), **self.optim_kwargs}
 
     def initialize(self, *args, **kwargs):
         super().initialize(*args, **kwargs)

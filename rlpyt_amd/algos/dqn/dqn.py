@@ -39,7 +39,7 @@ class DQN(RlAlgorithm):
                  ReplayBufferCls=None, updates_per_sync=1):
         hp = dict(locals())
         hp.pop("self")
-        hp["optim_kwargs"] = dict(eps=0.01 / batch_size) if optim_kwargs is None else optim_kwargs
+        hp["optim_kwargs"] = self.default_eps(OptimCls, 0.01 / batch_size) if optim_kwargs is None else optim_kwargs
         hp["default_priority"] = delta_clip if default_priority is None else default_priority
         self._batch_size = hp.pop("batch_size")
         self.__dict__.update(hp)

@@ -47,7 +47,7 @@ class R2D1(DQN):
                  value_scale_eps=1e-3, ReplayBufferCls=None, updates_per_sync=1):
         hp = dict(locals())
         hp.pop("self")
-        hp["optim_kwargs"] = dict(eps=1e-3) if optim_kwargs is None else optim_kwargs
+        hp["optim_kwargs"] = self.default_eps(OptimCls, 1e-3) if optim_kwargs is None else optim_kwargs
         hp["default_priority"] = (delta_clip or 1.) if default_priority is None else default_priority
         if input_priority_shift is None:      # priorities of a batch belong to sequences that
             hp["input_priority_shift"] = warmup_T // store_rnn_state_interval   # started earlier

@@ -195,3 +195,28 @@ def test_gradients_that_would_be_lost_are_refused(call):
         call(z(4, 4, requires_grad=True))
     with torch.no_grad(), pytest.raises((ValueError, _lib.HipError), match="device|MI355X"):     # (these are on the CPU)
         call(z(4, 4, requires_grad=True))
+
+
+def optimizer_of(algo):
+    params = [torch.nn.Parameter(z(3, 4)), torch.nn.Parameter(z(3))]
+    return algo.make_optimizer(params, algo.OptimCls, algo.learning_rate, algo.optim_kwargs)
+
+
+@pytest.mark.parametrize("given", [None, dict(momentum=0.5)])
+def test_algorithms_build_muon(given):
+    """Also those whose defaults are Adam's: its eps goes to the optimizers that have one."""
+    from rlpyt_amd.algos.dqn.cat_dqn import CategoricalDQN
+    from rlpyt_amd.algos.dqn.dqn import DQN
+    from rlpyt_amd.algos.dqn.r2d1 import R2D1
+    from rlpyt_amd.algos.pg.a2c import A2C
+    from rlpyt_amd.algos.pg.ppo import PPO
+    for Algo in (PPO, A2C, DQN, CategoricalDQN, R2D1):
+        kwargs = None if given is None else dict(given)
+        opt = optimizer_of(Algo(OptimCls=Muon, optim_kwargs=kwargs, learning_rate=0.02))
+        assert type(opt) is Muon and opt.param_groups[0]["momentum"] == (0.95 if given is None else 0.5)
+        assert kwargs == given                      # the caller's own dict stays as it was
+    for Algo, eps in ((DQN, 0.01 / 32), (CategoricalDQN, 0.01 / 32), (R2D1, 1e-3)):
+        for OptimCls in (torch.optim.Adam, torch.optim.AdamW, torch.optim.RMSprop):
+            assert optimizer_of(Algo(OptimCls=OptimCls)).param_groups[0]["eps"] == eps
+            assert optimizer_of(Algo(OptimCls=OptimCls, optim_kwargs=dict(eps=0.5))).param_groups[0]["eps"] == 0.5
+        assert "eps" not in optimizer_of(Algo(OptimCls=torch.optim.SGD)).param_groups[0]
