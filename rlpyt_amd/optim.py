@@ -302,12 +302,14 @@ class Muon(torch.optim.Optimizer):
     @torch.no_grad()
     def clip_and_step(self, max_norm, norm_out=None):
         """``clip_grad_norm_(params, max_norm)`` + ``step()``; returns the gradient norm before clipping
-        (device scalar).  ``max_norm`` None or <= 0: no clipping.  ``norm_out``: as in ``ClipAdam``."""
+        (device scalar).  ``max_norm`` None, <= 0 or infinite: no clipping (an infinite
+        gradient leaves the others alone).  ``norm_out``: as in ``ClipAdam``."""
         params = [p for g in self.param_groups for p in g["params"] if p.grad is not None]
         if not params:
             norm = torch.zeros((), device=self.param_groups[0]["params"][0].device)
+        elif max_norm and 0 < max_norm < math.inf:
+            norm = torch.nn.utils.clip_grad_norm_(params, float(max_norm))
         else:
-            bound = float(max_norm) if max_norm and max_norm > 0 else math.inf
-            norm = torch.nn.utils.clip_grad_norm_(params, bound)
+            norm = torch.nn.utils.get_total_norm([p.grad for p in params])
         self.step()
         return ClipAdam._to_out(norm, norm_out)

@@ -220,3 +220,19 @@ def test_algorithms_build_muon(given):
             assert optimizer_of(Algo(OptimCls=OptimCls)).param_groups[0]["eps"] == eps
             assert optimizer_of(Algo(OptimCls=OptimCls, optim_kwargs=dict(eps=0.5))).param_groups[0]["eps"] == 0.5
         assert "eps" not in optimizer_of(Algo(OptimCls=torch.optim.SGD)).param_groups[0]
+
+
+@pytest.mark.parametrize("max_norm", [None, 0., -1., float("inf")])
+def test_muon_without_a_bound_leaves_the_gradients(max_norm):
+    """An infinite gradient then stays in its own parameter; what is returned is the norm."""
+    a, b = (torch.nn.Parameter(torch.ones(3)) for _ in range(2))
+    a.grad, b.grad = torch.full((3,), 2.), torch.tensor([1., float("inf"), 1.])
+    norm = Muon([a, b], lr=0.02).clip_and_step(max_norm)
+    assert float(norm) == float("inf")
+    assert torch.equal(a.grad, torch.full((3,), 2.))
+    assert torch.allclose(a.detach(), torch.full((3,), 0.999))         # Adam's first step: lr x adam_lr_ratio
+    b.grad = torch.tensor([1., 2., 2.])
+    norm = Muon([a, b], lr=0.02).clip_and_step(max_norm)
+    assert abs(float(norm) - 21 ** 0.5) < 1e-6 and torch.equal(b.grad, torch.tensor([1., 2., 2.]))
+    norm = Muon([a, b], lr=0.02).clip_and_step(1.)
+    assert abs(float(norm) - 21 ** 0.5) < 1e-6 and abs(float(torch.cat([a.grad, b.grad]).norm()) - 1.) < 1e-5
