@@ -10,7 +10,8 @@ the C ABI (``include/rlpyt_hip.h``); ``rlpyt_amd.ops`` offers them with the othe
 Arguments that do not fit raise ``ValueError`` before anything is launched, tensors with a forward-mode derivative
 (``torch.autograd.forward_ad``) among them.  Kernels run on the current stream of the
 tensors' device; workspaces come from torch's allocator per call, so that captured graphs do not share them.  Behind the
-checks, the first four run in a small extension (``csrc/seqops.cpp``): allocations, launches and autograd nodes.
+checks, the first four run in a small extension (``csrc/seqops.cpp``, loaded by the first call): allocations, launches and autograd
+nodes.
 
 Small calls wait for autograd's device thread longer than for the device: a program with one GPU may run its backward passes
 under ``torch.autograd.set_multithreading_enabled(False)``, which halves a small scan's time.
@@ -27,15 +28,25 @@ from torch.autograd import forward_ad
 from . import _lib
 from ._lib import check, lib
 
-try:
-    from . import _seqops       # (after _lib: it takes the C entry points from the library that is loaded there)
-except ImportError as e:
-    raise _lib.HipExtensionMissing(
-        f"rlpyt_amd/_seqops.so cannot be loaded ({e}). Run `python -c 'import __graft_entry__ as g; g.build()'` (or "
-        "`make -C rlpyt_amd/csrc`).") from e
-if _seqops.abi_version != _lib.ABI_VERSION:
-    raise _lib.HipExtensionMissing(
-        f"rlpyt_amd/_seqops.so has ABI {_seqops.abi_version}, binding expects {_lib.ABI_VERSION}: rebuild.")
+class _Unloaded:
+    """Stands in for the extension until the first call that needs it: what does without these operators does without the file."""
+
+    def __getattr__(self, name):
+        global _seqops
+        try:
+            from . import _seqops as loaded   # (after _lib: it takes the C entry points from the library that is loaded there)
+        except ImportError as e:
+            raise _lib.HipExtensionMissing(
+                f"rlpyt_amd/_seqops.so cannot be loaded ({e}). Run `python -c 'import __graft_entry__ as g; g.build()'` (or "
+                "`make -C rlpyt_amd/csrc`).") from e
+        if loaded.abi_version != _lib.ABI_VERSION:
+            raise _lib.HipExtensionMissing(
+                f"rlpyt_amd/_seqops.so has ABI {loaded.abi_version}, binding expects {_lib.ABI_VERSION}: rebuild.")
+        _seqops = loaded
+        return getattr(loaded, name)
+
+
+_seqops = _Unloaded()
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _FLOATS = (torch.float32, torch.float64, torch.bfloat16, torch.float16)

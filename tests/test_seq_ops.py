@@ -4,6 +4,7 @@ import ctypes
 import os
 import shutil
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -236,3 +237,37 @@ def test_muon_without_a_bound_leaves_the_gradients(max_norm):
     assert abs(float(norm) - 21 ** 0.5) < 1e-6 and torch.equal(b.grad, torch.tensor([1., 2., 2.]))
     norm = Muon([a, b], lr=0.02).clip_and_step(1.)
     assert abs(float(norm) - 21 ** 0.5) < 1e-6 and abs(float(torch.cat([a.grad, b.grad]).norm()) - 1.) < 1e-5
+
+
+WITHOUT_EXTENSION = """
+import sys, types
+class Gone:
+    def find_spec(self, name, path=None, target=None):
+        if name == "rlpyt_amd._seqops":
+            raise ImportError("undefined symbol: of another torch")
+sys.meta_path.insert(0, Gone())
+from rlpyt_amd import _lib, ops, ops_seq, optim
+from rlpyt_amd.algos.dqn.r2d1 import R2D1
+from rlpyt_amd.algos.pg.ppo import PPO
+assert ops.orthogonalize([]) == [] and callable(ops.gae)
+stale = types.ModuleType("rlpyt_amd._seqops")
+stale.abi_version = _lib.ABI_VERSION - 1
+for wrong in ("cannot be loaded", "cannot be loaded", "rebuild"):
+    if wrong == "rebuild":
+        sys.modules["rlpyt_amd._seqops"] = stale
+    for use in (lambda: ops_seq._seqops.gated_scan, lambda: ops_seq._seqops.action_logp):
+        try:
+            use()
+        except _lib.HipExtensionMissing as e:
+            assert wrong in str(e), e
+        else:
+            raise SystemExit("used without the extension")
+"""
+
+
+def test_only_the_operators_that_use_the_extension_need_it():
+    """The rest of the package imports where ``_seqops.so`` is missing or was built against another torch; the operators behind
+    it fail loudly, every time."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(_lib.__file__)))
+    run = subprocess.run([sys.executable, "-c", WITHOUT_EXTENSION], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr
