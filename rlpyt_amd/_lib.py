@@ -55,6 +55,10 @@ class HipError(RuntimeError):
     pass
 
 
+class HipArgumentError(HipError, ValueError):
+    """An argument that the library refuses by itself."""
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise HipExtensionMissing(

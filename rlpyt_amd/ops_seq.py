@@ -21,6 +21,7 @@ drop eager results that still hang on the same leaves (their nodes belong to the
 input is such a leaf raises ``RuntimeError``).
 """
 import ctypes
+import functools
 
 import torch
 from torch.autograd import forward_ad
@@ -254,6 +255,14 @@ def action_logp(logits, action):
 NS_COEFFS = (3.4445, -4.7750, 2.0315)
 
 
+@functools.lru_cache(maxsize=64)
+def _check_polynomial(steps, a, b, c):
+    """The library's own check of the polynomial, which comes before the matrices: here an empty one."""
+    none, pointer = (ctypes.c_int64 * 1)(0), (ctypes.c_void_p * 1)(None)
+    if lib.rlpyt_orthogonalize(0, pointer, none, pointer, none, none, 1, steps, a, b, c, 0., None, None):
+        raise _lib.HipArgumentError(_lib.last_error())
+
+
 def orthogonalize(mats, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     """Newton-Schulz orthogonalisation of an update: ``X = G / (|G|_F + eps)``, then ``steps`` times ``X <-
     a X + (b A + c A A) X`` with ``A = X X^T`` (of the wide form), which moves the singular values towards 1 and keeps
@@ -266,12 +275,14 @@ def orthogonalize(mats, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     require a gradient are taken under ``torch.no_grad()`` only."""
     single = isinstance(mats, torch.Tensor)
     mats = [mats] if single else list(mats)
-    if int(steps) != steps or not 1 <= steps <= 100:
+    if not 1 <= steps <= 100 or int(steps) != steps:
         _refuse(f"orthogonalize: 1 to 100 steps are needed, got {steps}")
     if len(coeffs) != 3:
         _refuse("orthogonalize: three coefficients are needed")
     if not eps >= 0.:
         _refuse("orthogonalize: eps >= 0 is needed")
+    steps, coeffs = int(steps), [float(v) for v in coeffs]
+    _check_polynomial(steps, *coeffs)
     for g in mats:
         if g.dim() < 2 or g.dtype not in _DTYPES:
             _refuse(f"orthogonalize: matrices in float32, bfloat16 or float16 are needed, got {tuple(g.shape)} {g.dtype}")
@@ -309,7 +320,7 @@ def orthogonalize(mats, steps=5, coeffs=NS_COEFFS, eps=1e-7):
         lds, rows, cols = ((ctypes.c_int64 * k)(*v) for v in (lds, rows, cols))
         ws = torch.empty(lib.rlpyt_orthogonalize_workspace_bytes(rows, cols, k), dtype=torch.uint8, device=device)
         with torch.cuda.device(device):
-            check(lib.rlpyt_orthogonalize(_DTYPES[dtype], ins, lds, dsts, rows, cols, k, int(steps), *map(float, coeffs),
+            check(lib.rlpyt_orthogonalize(_DTYPES[dtype], ins, lds, dsts, rows, cols, k, steps, *coeffs,
                                           float(eps), ws.data_ptr(), torch.cuda.current_stream().cuda_stream),
                   "rlpyt_orthogonalize")
     return outs[0] if single else outs

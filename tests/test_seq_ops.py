@@ -271,3 +271,17 @@ def test_only_the_operators_that_use_the_extension_need_it():
     root = os.path.dirname(os.path.dirname(os.path.abspath(_lib.__file__)))
     run = subprocess.run([sys.executable, "-c", WITHOUT_EXTENSION], cwd=root, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stderr
+
+
+@pytest.mark.parametrize("options", [dict(coeffs=(9., 0., 0.)), dict(coeffs=(3., 0., 3.)), dict(coeffs=(float("nan"), 0., 0.)),
+                                     dict(coeffs=(2., float("inf"), 0.)), dict(steps=float("inf")), dict(steps=float("nan"))])
+def test_orthogonalize_refuses_its_options_as_arguments(options):
+    """As ValueError like every argument that does not fit, and first of all: before the matrices are looked at."""
+    for mats in (z(4, 4), [z(4, 4), z(2, 3, 5)], []):
+        with pytest.raises(ValueError):
+            ops.orthogonalize(mats, **options)
+
+
+def test_orthogonalize_takes_bounded_options():
+    for steps, coeffs in ((5, (3.4445, -4.7750, 2.0315)), (100, (1.5, -0.5, 0.)), (3., (2., -1.5, 0.5))):
+        assert ops.orthogonalize([], steps=steps, coeffs=coeffs) == []
