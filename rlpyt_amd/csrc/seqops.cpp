@@ -80,11 +80,12 @@ void check_leaves(const char* what, std::initializer_list<const Tensor*> inputs)
 }
 
 // ---- gated linear recurrence ------------------------------------------------------------------------------
-// An empty [T, B, D] whose rows lie in memory in the order of x's: time or batch first.
+// An empty [T, B, D] whose rows lie in memory in the order of x's: time or batch first.  (By its strides: a transposed view made
+// under a node could not be written in place.)
 Tensor like_rows(const Tensor& x) {
   if (x.is_contiguous()) return at::empty_like(x);
   const int64_t T = x.size(0), B = x.size(1), D = x.size(2);
-  if (T > 1 && B > 1 && x.stride(1) > x.stride(0)) return at::empty({B, T, D}, x.options()).transpose(0, 1);
+  if (T > 1 && B > 1 && x.stride(1) > x.stride(0)) return at::empty_strided({T, B, D}, {D, T * D, 1}, x.options());
   return at::empty({T, B, D}, x.options());
 }
 

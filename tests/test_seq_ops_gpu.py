@@ -1019,3 +1019,18 @@ def test_policy_kl_loss_of_an_empty_batch(V):
         assert float(loss) == 0. and not bool(scalars.any())
     lp, ent = ops.action_logp(logits.detach(), none.long())
     assert lp.shape == (0,) and ent.shape == (0,)
+
+
+@pytest.mark.parametrize("layout", ["dense", "batch first", "halves", "odd start"])
+def test_gated_scan_results_may_be_written_in_place(layout):
+    """As any operator's: the states are a tensor of their own, also where they lie in memory like a [B, T, D] input."""
+    x, gate, h0, dh, dhn, rs, ln = scan_data(70, 3, 34, torch.float32, 150, True, True, layout)
+    plain = scan_grads(x, gate, h0, dh, dhn, rs, ln)
+    leaves = [t.detach().requires_grad_(True) for t in (x, gate, h0)]
+    h, hn = ops.gated_scan(*leaves, reset=rs, lengths=ln)
+    h.mul_(2.)
+    hn.add_(1.)
+    assert torch.equal(h.detach(), 2. * plain["h"].detach()) and torch.equal(hn.detach(), plain["hn"].detach() + 1.)
+    grads = torch.autograd.grad((h, hn), leaves, (dh, dhn))
+    again = torch.autograd.grad(ops.gated_scan(*leaves, reset=rs, lengths=ln), leaves, (2. * dh, dhn))
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
