@@ -101,7 +101,10 @@ __device__ __forceinline__ double log_of(float s) {
 }
 // e^d - d - 1 >= 0, to ~ 2^-20 relative: the series where it cancels
 __device__ __forceinline__ double kl_of(double d) {
-  if (fabs(d) > 0.5) return (double)expf((float)d) - d - 1.0;
+  if (fabs(d) > 0.5) {
+    const double e = (double)expf((float)d);
+    return e == INFINITY ? e : e - d - 1.0;   // (d may be infinite itself)
+  }
   double v = 1.0;                     // d^12 / 12! is left out
 #pragma unroll
   for (int k = 11; k >= 3; --k) v = fma(v, d * (1.0 / k), 1.0);
@@ -158,7 +161,7 @@ __device__ __forceinline__ RowOut row_terms(const LossArgs& p, int64_t n, float 
   if (p.ref_logp) {
     const double d = (double)p.ref_logp[n] - lp;
     o.kl = kl_of(d);
-    c -= p.c_kl * (o.kl + d);
+    c -= p.c_kl * (d == -INFINITY ? -1.0 : o.kl + d);   // e^d - 1
   }
   o.ent = H;
   const double g = denom > 0.0 ? p.g_scale * (double)w / denom : 0.0, gs = g / (double)st.s;

@@ -215,7 +215,8 @@ def policy_kl_loss(logits, action, old_logp, advantage, ref_logp=None, valid=Non
     Logits of -inf are actions that are not allowed.  Rows whose ``valid`` is 0 are not read and have a zero
     gradient, also where their action is out of range; nothing valid gives a loss of 0.  A row that allows
     no action adds 0 and has a zero gradient, but counts in the mean.  In a valid row an action outside 0 .. V-1 or a NaN
-    logit makes the loss NaN; with a KL term, so does the gradient of an action that is not allowed (its kl is infinite)."""
+    logit makes the loss NaN.  The kl of an action that is not allowed is infinite, and so is a loss with a KL term; the
+    row's gradient is NaN then."""
     lead = logits.shape[:-1]
     for name, t in (("old_logp", old_logp), ("advantage", advantage), ("ref_logp", ref_logp), ("valid", valid)):
         if t is None and name in ("ref_logp", "valid"):

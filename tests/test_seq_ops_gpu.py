@@ -1034,3 +1034,22 @@ def test_gated_scan_results_may_be_written_in_place(layout):
     grads = torch.autograd.grad((h, hn), leaves, (dh, dhn))
     again = torch.autograd.grad(ops.gated_scan(*leaves, reset=rs, lengths=ln), leaves, (2. * dh, dhn))
     assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
+@pytest.mark.parametrize("V", [7, 18, 100, 500, 3000, 20000, 140000])
+def test_policy_kl_loss_infinite_kl(V):
+    """An action that is not allowed, of a finite log-probability under the reference policy, and one the other way round."""
+    logits, action, old, adv, ref, _ = loss_data(12, V, torch.float32, 161)
+    none = logits.clone()
+    none[2, action[2]] = -math.inf
+    never = ref.clone()
+    never[5] = -math.inf
+    for data in ((none, action, old, adv, ref, None), (logits, action, old, adv, never, None)):
+        loss, scalars, grad = run_loss(*data, kl_coeff=0.1, **KW)
+        assert float(loss) == math.inf and float(scalars[2]) == math.inf
+        assert bool(torch.isfinite(scalars[[1, 3, 4]]).all())
+        if data[4] is never:                 # e^d - 1 = -1
+            _, want = loss64(*data, 0.2, 0.3, 0.1)
+            err = (64 + 4) * 2. ** -24 + 2. ** -20         # as in loss_close
+            assert bool(((grad.double() - want).abs() <= 2. ** -24 * want.abs()
+                         + 4 * err * want.abs().amax(-1, keepdim=True)).all())
