@@ -861,8 +861,8 @@ int rlpyt_gated_scan_step(int dtype, const void* x, int64_t x_bs, const void* ga
  *   loss = sum valid (pi + kl_coeff (e^d - d - 1) - entropy_coeff H) / sum valid
  * ref_logp, valid (f32 weights; rows of weight 0 are not read) may be null.  scalars [5] = loss (also
  * in *loss), pi, kl, entropy and clipped share (weighted means; 0 when nothing is valid).  grad [N,V] dense (may be null): grad_scale d loss /
- * d logits.  A row of -inf only adds nothing; an action
- * outside 0 .. V-1 makes the loss NaN. */
+ * d logits.  A row of -inf only adds nothing; an action outside 0 .. V-1 makes the loss NaN.  With kl_coeff = 0 the kl goes
+ * to scalars only, whatever it is. */
 int64_t rlpyt_policy_loss_workspace_bytes(int dtype, int64_t N, int64_t V);
 int rlpyt_policy_kl_loss_fwd_bwd(int dtype, const void* logits, int64_t row_stride, const int64_t* action,
                                  const float* old_logp, const float* advantage, const float* ref_logp,

@@ -216,7 +216,8 @@ def policy_kl_loss(logits, action, old_logp, advantage, ref_logp=None, valid=Non
     gradient, also where their action is out of range; nothing valid gives a loss of 0.  A row that allows
     no action adds 0 and has a zero gradient, but counts in the mean.  In a valid row an action outside 0 .. V-1 or a NaN
     logit makes the loss NaN.  The kl of an action that is not allowed is infinite, and so is a loss with a KL term; the
-    row's gradient is NaN then."""
+    row's gradient is NaN then.  With ``kl_coeff`` = 0 a reference policy is watched only: ``scalars`` has its kl, the loss and
+    the gradient have nothing of it."""
     lead = logits.shape[:-1]
     for name, t in (("old_logp", old_logp), ("advantage", advantage), ("ref_logp", ref_logp), ("valid", valid)):
         if t is None and name in ("ref_logp", "valid"):

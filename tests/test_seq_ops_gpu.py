@@ -1053,3 +1053,24 @@ def test_policy_kl_loss_infinite_kl(V):
             err = (64 + 4) * 2. ** -24 + 2. ** -20         # as in loss_close
             assert bool(((grad.double() - want).abs() <= 2. ** -24 * want.abs()
                          + 4 * err * want.abs().amax(-1, keepdim=True)).all())
+
+
+@pytest.mark.parametrize("V", [7, 18, 100, 500, 3000, 20000, 140000])
+def test_policy_kl_loss_without_weight_on_the_kl_term(V):
+    """A reference policy that is only watched (kl_coeff = 0): where e^d is beyond 32 bits, kl is infinite, the loss and its
+    gradient are those without a reference policy."""
+    logits, action, old, adv, ref, w = loss_data(12, V, torch.float32, 160)
+    far = ref.clone()
+    far[2], w[2] = 100., 1.
+    c = dict(entropy_coeff=0.02, **KW)
+    loss, scalars, grad = run_loss(logits, action, old, adv, None, w, **c)
+    got_loss, got, got_grad = run_loss(logits, action, old, adv, far, w, **c)
+    assert torch.equal(got_loss, loss) and torch.equal(got_grad, grad) and float(got[2]) == math.inf
+    assert torch.equal(got[[0, 1, 3, 4]], scalars[[0, 1, 3, 4]])
+    # an action that is not allowed: log-probability -inf, ratio 0, kl infinite
+    none = logits.clone()
+    none[2, action[2]] = -math.inf
+    loss, scalars, grad = run_loss(none, action, old, adv, None, w, **c)
+    got_loss, got, got_grad = run_loss(none, action, old, adv, ref, w, **c)
+    assert math.isfinite(float(loss)) and torch.equal(got_loss, loss) and torch.equal(got_grad, grad)
+    assert float(got[2]) == math.inf
