@@ -533,14 +533,17 @@ int channels(int size, int64_t D) { return size == 2 && D > 1 ? 2 : 1; }
 int64_t tiles_of(int64_t B, int64_t D, int V) { return ceil_div(B * ceil_div(D, V), kWave); }
 
 // W: waves that share the channels of one tile: 4 where the tiles fill the chip, else 8 (or what T needs).  S: segments
-// along time.  A single segment reads the streams once; S > 1 reads them twice and adds a launch, so it is taken only where
-// the tiles alone leave many of the 256 CUs idle (128 tiles of 2048 steps: 190 us in one segment, 175 in four).
+// along time.  A single segment reads the streams once; S > 1 reads them twice and adds a launch each way, so it needs idle CUs
+// and windows that S segments take off the chain.  Both directions in f32 (bf16), one segment -> split: 48 tiles of 128 steps 12.6 ->
+// 16.1 us (15.5 -> 18.8), of 256 20.5 -> 16.9 (26.5 -> 20.0); 64 of 256 21.0 -> 17.7 (26.7 -> 20.5); 96 of 256 21.9 -> 22.8 (27.9 -> 31), of
+// 512 38.3 -> 36.4 (49.7 -> 50.2), of 1024 69 -> 56 (92 -> 73); 128 of 512 38.3 -> 40.9 (49.8 -> 54.6), of 1024 69 -> 69 (92 -> 88),
+// of 2048 145 -> 134 (179 -> 157); 144 of 2048 153 -> 175 (184 -> 218).
 Plan plan_of(int64_t T, int64_t tiles) {
   Plan q;
   q.W = (int)std::min<int64_t>(tiles >= 512 ? 4 : kMaxWaves, std::max<int64_t>(1, ceil_div(T, kL)));
   const int64_t window = (int64_t)q.W * kL, windows = std::max<int64_t>(1, ceil_div(T, window));
   int64_t S = 1;
-  if (tiles < 192) S = std::min<int64_t>({windows, ceil_div(512, tiles), (int64_t)256});
+  if (tiles <= 128 && windows >= (tiles <= 64 ? 4 : tiles <= 96 ? 8 : 16)) S = std::min<int64_t>({windows, ceil_div(512, tiles), (int64_t)256});
   const int64_t seg = ceil_div(windows, S) * window;
   q.S = (int)std::max<int64_t>(1, ceil_div(T, seg));
   q.seg = (int)std::min<int64_t>(seg, (int64_t)1 << 30);

@@ -285,3 +285,13 @@ def test_orthogonalize_refuses_its_options_as_arguments(options):
 def test_orthogonalize_takes_bounded_options():
     for steps, coeffs in ((5, (3.4445, -4.7750, 2.0315)), (100, (1.5, -0.5, 0.)), (3., (2., -1.5, 0.5))):
         assert ops.orthogonalize([], steps=steps, coeffs=coeffs) == []
+
+
+@pytest.mark.parametrize("T,channels,split", [
+    (64, 1, False), (85, 16 * 512, False), (128, 16 * 512, False), (192, 64, False), (256, 64, True), (256, 64 * 64, True),
+    (448, 80 * 64, False), (512, 80 * 64, True), (960, 112 * 64, False), (1024, 112 * 64, True), (1 << 16, 128 * 64, True),
+    (2048, 144 * 64, False), (1 << 16, 160 * 64, False), (1 << 16, 512, True),
+])
+def test_where_time_is_split(T, channels, split):
+    """Segments of time (whose maps are the workspace) need steps enough to pay for their launch and their second read."""
+    assert (_lib.lib.rlpyt_gated_scan_workspace_bytes(T, channels, 1) > 0) == split    # D = 1: 64 channels a tile in every type
