@@ -692,8 +692,10 @@ extern "C" int rlpyt_policy_kl_loss_fwd_bwd(int dtype, const void* logits, int64
   p.ref_logp = ref_logp, p.valid = valid, p.grad = grad;
   double *denom = (double*)workspace, *shares = (double*)((char*)workspace + 16);
   p.rows = (double*)((char*)workspace + kRowsOffset);
-  // The sum of the weights: by every workgroup where that is few numbers altogether, else in a launch of its own.  (8192 x 18: 17 us
-  // on the device either way, and 4 us less of the call.)
+  // The sum of the weights: by every workgroup where that is few numbers altogether, else in a launch of its own, which costs 4 us of
+  // the call.  On the device, f32 without a gradient, by every workgroup and in a launch: 1024 x 18 11.7 and 12.1 us, 8192 x 18 12.0 and
+  // 12.0, 16384 x 18 13.4 and 12.7, 30000 x 18 19.0 and 16.1; 2048 x 500 10.7 and 11.1, 4096 x 500 12.4 and 12.1; 1024 x 3000 12.2 and
+  // 12.3, 2048 x 3000 15.3 and 14.7.
   const bool fold = q.groups(N) * N <= (int64_t)1 << 21;
   p.denom = valid && !fold ? denom : nullptr;
   p.parts = (Stats*)((char*)workspace + parts_offset(q));

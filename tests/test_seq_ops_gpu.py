@@ -1074,3 +1074,26 @@ def test_policy_kl_loss_without_weight_on_the_kl_term(V):
     got_loss, got, got_grad = run_loss(none, action, old, adv, ref, w, **c)
     assert math.isfinite(float(loss)) and torch.equal(got_loss, loss) and torch.equal(got_grad, grad)
     assert float(got[2]) == math.inf
+
+
+def test_gated_scan_accuracy_of_the_gates():
+    """z from one step out of 0 (h = z x with x = 1), 1 - z from one step out of 1 (x = 0).  In units of 2^-24: the exponent g log2(e) is
+    rounded once (|g|) with a rounded factor (0.22 |g|), exp2 2, 1 + e 1, the reciprocal 1, a product 1; in the larger of z and 1 - z the
+    exponent's part is weighed down by the smaller."""
+    g = torch.linspace(-60., 60., 1 << 16, device=DEV).view(1, 1, -1)
+    one, zero = torch.ones_like(g), torch.zeros_like(g)
+    for got, want in ((ops.gated_scan(one, g, zero[0])[0], torch.sigmoid(g.double())),
+                      (ops.gated_scan(zero, g, one[0])[0], torch.sigmoid(-g.double()))):
+        units = torch.where(want >= 0.5, 5., 1.3 * g.abs() + 5.)
+        assert bool(((got.double() / want - 1.).abs() <= units.double() * 2. ** -24).all())
+
+
+def test_orthogonalize_does_not_depend_on_the_run():
+    """Products split over their sums among them, and memory that holds something else each time."""
+    for sizes, dtype in ((((512, 3456), (18, 512), (32, 256)), torch.float32), (((1601, 1700),), torch.bfloat16)):
+        mats = [torch.randn(*s, device=DEV, generator=gen(170)).to(dtype) for s in sizes]
+        first = ops.orthogonalize(mats)
+        for k in range(3):
+            torch.full((1 << 26,), math.nan, device=DEV)          # (freed at once: the next workspace lies there)
+            ops.orthogonalize([m + k + 1 for m in mats])
+            assert all(torch.equal(a, b) for a, b in zip(ops.orthogonalize(mats), first))
