@@ -164,7 +164,7 @@ __device__ __forceinline__ RowOut row_terms(const LossArgs& p, int64_t n, float 
     if (p.c_kl != 0.0) c -= p.c_kl * (d == -INFINITY ? -1.0 : o.kl + d);   // e^d - 1
   }
   o.ent = H;
-  const double g = denom > 0.0 ? p.g_scale * (double)w / denom : 0.0, gs = g / (double)st.s;
+  const double g = denom != 0.0 ? p.g_scale * (double)w / denom : 0.0, gs = g / (double)st.s;
   o.k1 = (float)(gs * p.c_ent * kLn2);
   o.k0 = (float)(gs * (p.c_ent * (H - logs) - c));
   o.ka = (float)(g * c);
@@ -572,7 +572,7 @@ __global__ __launch_bounds__(1024) void loss_finish_kernel(const double* __restr
     for (int k = 0; k < 4; ++k) v[k] += rows[i * 4 + k];
   block_sum<4>(v, scratch);
   if (threadIdx.x != 0) return;
-  const double inv = d > 0.0 ? 1.0 / d : 0.0;   // nothing valid: a loss of 0
+  const double inv = d != 0.0 ? 1.0 / d : 0.0;   // nothing valid: a loss of 0
   for (int k = 0; k < 4; ++k) v[k] *= inv;
   *loss = scalars[0] = (float)(v[0] + (c_kl != 0.0 ? c_kl * v[1] : 0.0) - c_ent * v[2]);
   for (int k = 0; k < 4; ++k) scalars[1 + k] = (float)v[k];

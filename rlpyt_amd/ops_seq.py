@@ -202,7 +202,8 @@ def policy_kl_loss(logits, action, old_logp, advantage, ref_logp=None, valid=Non
 
     ``logits [..., V]`` float32, bfloat16 or float16, any row stride; ``action [...]`` whole numbers;
     ``old_logp, advantage, ref_logp [...]`` (the log-probabilities as ``action_logp`` gives them) and ``valid
-    [...]`` (weights, or a mask) are taken as float32 and as constants.  ``mean_valid`` divides by the sum of ``valid``.
+    [...]`` (weights, or a mask) are taken as float32 and as constants.  ``mean_valid`` divides by the sum of ``valid``, of
+    either sign; a sum of 0 gives 0.
 
     Returns ``(loss, scalars)``: ``loss`` is differentiable w.r.t. ``logits`` (one backward pass a call: the
     gradient comes out of the forward pass, is scaled in place and handed on), ``scalars = [loss, pi_loss, kl,

@@ -1097,3 +1097,23 @@ def test_orthogonalize_does_not_depend_on_the_run():
             torch.full((1 << 26,), math.nan, device=DEV)          # (freed at once: the next workspace lies there)
             ops.orthogonalize([m + k + 1 for m in mats])
             assert all(torch.equal(a, b) for a, b in zip(ops.orthogonalize(mats), first))
+
+
+@pytest.mark.parametrize("V", [18, 100, 500, 3000, 20000, 140000])
+def test_policy_kl_loss_weights_of_any_sign(V):
+    """The mean divides by the sum of the weights, whatever its sign; a NaN among them shows in the gradient too."""
+    logits, action, old, adv, ref, w = loss_data(14, V, torch.float32, 162)
+    w = torch.where(torch.arange(14, device=DEV) % 3 == 0, 0.25 * (w + 0.1), -(w + 0.1))
+    w[4] = 0.
+    c = dict(kl_coeff=0.1, entropy_coeff=0.02)
+    out = run_loss(logits, action, old, adv, ref, w, **KW, **c)
+    want_s, want_g = loss64(logits, action, old, adv, ref, w, 0.2, 0.3, 0.1, 0.02)
+    err = 4 * ((64 + 4) * 2. ** -24 + 2. ** -20)         # as in loss_close, of the terms, which cancel here by as much as the weights do
+    cancel = float(w.double().abs().sum() / w.double().sum().abs())
+    assert bool(((out[1].double() - want_s).abs() <= err * cancel * (want_s.abs().max() + 4 * math.log(V))).all()), (out[1], want_s)
+    assert bool(((out[2].double() - want_g).abs() <= err * want_g.abs().amax(-1, keepdim=True)).all())
+    same = run_loss(logits, action, old, adv, ref, -w, **KW, **c)
+    assert torch.equal(same[1], out[1]) and torch.equal(same[2], out[2])
+    w[5] = math.nan
+    loss, _, grad = run_loss(logits, action, old, adv, ref, w, **KW, **c)
+    assert math.isnan(float(loss)) and bool(torch.isnan(grad[w != 0]).all()) and not bool(grad[4].any())
