@@ -18,7 +18,8 @@ under ``torch.autograd.set_multithreading_enabled(False)``, which halves a small
 
 A backward pass that is captured into a graph needs what all of torch's autograd needs there: warm up on a side stream, and
 drop eager results that still hang on the same leaves (their nodes belong to the other stream; an operator whose own
-input is such a leaf raises ``RuntimeError``).
+input is such a leaf raises ``RuntimeError``, in its captured forward pass already; without a backward pass it is captured under
+``torch.no_grad()``).
 """
 import ctypes
 import functools
